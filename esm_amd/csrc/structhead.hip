@@ -19,6 +19,9 @@ namespace {
 // ------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void dim6_frames_kernel(const float* __restrict__ proj, int ldp, float trans_scale,
                                                           float* __restrict__ affine, float* __restrict__ bb, int M) {
+    // No fused multiply-adds here: (p trans_scale) + x / nx has to be rounded twice, as the reference rounds it, or a zero
+    // direction (x + t - t = 0) turns into the rounding error of t and decides the frame.
+#pragma clang fp contract(off)
     const int r = blockIdx.x * 256 + threadIdx.x;
     if (r >= M) return;
     const float* p = proj + (size_t)r * ldp;
