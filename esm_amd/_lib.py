@@ -79,6 +79,19 @@ SIGNATURES = {
     "esmk_attn_plan": (C.c_int, [vp, C.c_int, vp, C.c_int]),
     "esmk_attn_varlen": (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "esmk_attn_l64_d128": (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp]),
+    "esmk_layernorm_fwd": (C.c_int, [vp, C.c_int, C.c_int64, vp, vp, vp, vp, C.c_int, C.c_int, C.c_float, vp]),
+    "esmk_layernorm_bwd_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "esmk_layernorm_bwd": (C.c_int, [vp, C.c_int64, vp, C.c_int64, C.c_int, vp, vp, vp, vp, vp, vp, C.c_size_t, C.c_int,
+                                     C.c_int, vp]),
+    "esmk_attn_varlen_fwd": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                       C.c_float, vp]),
+    "esmk_attn_varlen_bwd_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "esmk_attn_varlen_bwd": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int,
+                                       C.c_int, C.c_float, vp, C.c_size_t, vp]),
+    "esmk_pref_loss_saved_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "esmk_pref_loss_fwd": (C.c_int, [vp, C.c_int, vp, vp, C.c_int, vp, C.c_double, C.c_double, C.c_double, C.c_int, C.c_int,
+                                     vp, C.c_size_t, vp, vp, vp]),
+    "esmk_pref_loss_bwd": (C.c_int, [vp, C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, vp]),
     "esmk_embed": (C.c_int, [vp, vp, C.c_int, vp, C.c_int, C.c_int, vp]),
     "esmk_esm3_encode": (C.c_int, [C.POINTER(EsmkEsm3Encoder), vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_int, C.c_int, vp]),
     "esmk_frames": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, vp]),

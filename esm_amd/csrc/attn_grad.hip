@@ -1,0 +1,657 @@
+// Block-diagonal (varlen packed, non-causal) attention for training, head dim 64 or 128: a forward pass that leaves the
+// log-sum-exp of every query row, and a backward pass that recomputes the probabilities from it.
+//
+//   S = scale Q K^T (masked keys: -inf),  P = exp(S - lse),  O = P V
+//   delta = rowsum(dO O),  dS = P (dO V^T - delta),  dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Query heads share key heads in groups of n_heads / n_kv_heads.  A query row without any key gets O = 0, lse = -inf and
+// no gradient; tokens before the first and behind the last sequence get zeros (lse -inf).
+//
+// Matrix products run on v_mfma_f32_32x32x16_bf16 with fp32 accumulators.  A product's operand that lives in the lanes is
+// held in registers for the whole kernel (queries in the forward and dQ kernels, keys in the dK / dV kernel); the other
+// side streams through a two-slot LDS ring of 64-row tiles, filled by LDS-DMA one tile ahead.  Scores are formed with the
+// resident side on the lanes and the streamed side in the registers, so the exponentiated tile converts in place (bf16,
+// the second operand of the MFMA that consumes it) and softmax statistics stay in fp32.  The transposed operand of the
+// second product is read from the same row-major tile with ds_read_b64_tr_b16: the LDS image's 16-byte chunks are
+// XOR-swizzled by a function of the row that keeps both the row reads and the transposed reads free of bank conflicts.
+//
+// The backward pass is two kernels, each with one owner for every output element (no atomics, so the same inputs give the
+// same bits): dQ per query block (three products; it also forms delta), dK / dV per key block (four).
+#include <math.h>
+
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace {
+
+constexpr int TR = 64;       // rows of a streamed tile
+constexpr int AG_WAVES = 4;
+constexpr float AG_LOG2E = 1.4426950408889634f, AG_LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
+
+// A strided [token][head][D] tensor, strides in elements.
+struct View {
+    const __bf16* p;
+    int64_t tok, head;
+};
+struct OutView {
+    __bf16* p;
+    int64_t tok, head;
+};
+
+// ---- LDS image of a 64-row tile: row r at r * 2D bytes, its 16-byte chunk c at c ^ swz(r) -----------------------------
+//   row reads (32 rows, one logical chunk, ds_read_b128): 16 consecutive rows cover all 64 banks
+//   transposed reads (rows 4h..4h+3, 64 bytes each, ds_read_b64_tr_b16): the four rows cover all 64 banks
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+    if constexpr (D == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1);  // bit reversal of (r >> 1) & 7
+    else return (r & 3) << 2 | ((r >> 2) & 3);
+}
+
+// LDS-DMA of one tile: a wave moves pieces of 1 KiB (64 lanes x 16 bytes, LDS side linear, swizzle on the source address).
+// Rows past `rows` are out of the descriptor's range and land as zeros.
+template <int D>
+struct Stage {
+    static constexpr int RB = 2 * D, CPR = D / 8, PIECES = TR * RB / 1024 / AG_WAVES;
+    unsigned off[PIECES];
+    unsigned ldb;
+    __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
+        ldb = (unsigned)(ld * 2);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = (wave * PIECES + i) * (64 / CPR) + lane / CPR;
+            off[i] = (unsigned)r * ldb + (unsigned)((lane & (CPR - 1)) ^ swz<D>(r)) * 16u;
+        }
+    }
+    // first: first row of the tile (wave-uniform), rows: rows of it that exist (>= 1)
+    __device__ __forceinline__ void go(char* lds, const __bf16* first, int rows, int wave) const {
+        const int nrec = (int)((rows < TR ? rows - 1 : TR - 1) * ldb + RB);
+        const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, nrec, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(d, LDS_PTR(lds + (wave * PIECES + i) * 1024), 16, (int)off[i], 0, 0, 0);
+    }
+};
+
+// Transposed fragments (first operand of an MFMA over 16 tile rows) of all D / 32 column tiles, for 16-row step SP and, at
+// D = 64, also SP + 1: eight ds_read_b64_tr_b16.  Fragment slot (hi, j) holds tile row 16 SP + 4 hi + (j & 3) + 8 (j >> 2),
+// which is the row of accumulator register 8 (SP & 1) + j: the converted scores are the second operand as they stand.
+// The wait is part of the statement: no load is in flight when the compiler sees its outputs.
+template <int D>
+struct TrAddr {
+    unsigned a[2][D / 32];  // [rows +0 / +8][column tile], bytes inside a tile
+    __device__ __forceinline__ void init(int lane) {
+        const int i = lane & 15, g = (lane >> 4) & 1, hi = lane >> 5;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 4 * hi + (i >> 2) + 8 * e, ch = 2 * g + ((i & 3) >> 1);
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t) a[e][t] = (unsigned)(r * 2 * D + (((4 * t + ch) ^ swz<D>(r)) << 4) + (i & 1) * 8);
+        }
+    }
+};
+struct TrFrag { u32x2 v[8]; };
+
+#define AG_TR8(F, A0, A1, A2, A3, A4, A5, A6, A7, O0, O1)                                                               \
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%c16\n\tds_read_b64_tr_b16 %1, %9 offset:%c16\n\t"                    \
+                 "ds_read_b64_tr_b16 %2, %10 offset:%c16\n\tds_read_b64_tr_b16 %3, %11 offset:%c16\n\t"                  \
+                 "ds_read_b64_tr_b16 %4, %12 offset:%c17\n\tds_read_b64_tr_b16 %5, %13 offset:%c17\n\t"                  \
+                 "ds_read_b64_tr_b16 %6, %14 offset:%c17\n\tds_read_b64_tr_b16 %7, %15 offset:%c17\n\t"                  \
+                 "s_waitcnt lgkmcnt(0)"                                                                                 \
+                 : "=&v"(F.v[0]), "=&v"(F.v[1]), "=&v"(F.v[2]), "=&v"(F.v[3]), "=&v"(F.v[4]), "=&v"(F.v[5]),             \
+                   "=&v"(F.v[6]), "=&v"(F.v[7])                                                                         \
+                 : "v"(A0), "v"(A1), "v"(A2), "v"(A3), "v"(A4), "v"(A5), "v"(A6), "v"(A7), "i"(O0), "i"(O1)              \
+                 : "memory")
+
+// D = 64: v[4 s + 2 t + e] for 16-row steps SP + s; D = 128: v[2 t + e] for step SP
+template <int D, int SP>
+__device__ __forceinline__ TrFrag tr_read(const TrAddr<D>& ta, unsigned tile) {
+    TrFrag f;
+    constexpr int O = SP * 16 * 2 * D;
+    if constexpr (D == 64) {
+        const unsigned a0 = tile + ta.a[0][0], a1 = tile + ta.a[1][0], a2 = tile + ta.a[0][1], a3 = tile + ta.a[1][1];
+        AG_TR8(f, a0, a1, a2, a3, a0, a1, a2, a3, O, O + 16 * 2 * D);
+    } else {
+        AG_TR8(f, tile + ta.a[0][0], tile + ta.a[1][0], tile + ta.a[0][1], tile + ta.a[1][1], tile + ta.a[0][2],
+               tile + ta.a[1][2], tile + ta.a[0][3], tile + ta.a[1][3], O, O);
+    }
+    return f;
+}
+__device__ __forceinline__ bf16x8 tr_frag(const TrFrag& f, int i) {
+    return __builtin_bit_cast(bf16x8, u32x4{f.v[i].x, f.v[i].y, f.v[i + 1].x, f.v[i + 1].y});
+}
+
+// acc[t] (column tile t of D, lanes = resident rows) += X^T . B, X = tile rows 32 MT .. 32 MT + 31, b = their two 16-row steps
+template <int D, int MT>
+__device__ __forceinline__ void mfma_tr(f32x16 (&acc)[D / 32], const TrAddr<D>& ta, unsigned tile, const bf16x8 (&b)[2]) {
+    if constexpr (D == 64) {
+        const TrFrag f = tr_read<D, 2 * MT>(ta, tile);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag(f, 4 * s + 2 * t), b[s], acc[t], 0, 0, 0);
+    } else {
+        {
+            const TrFrag f = tr_read<D, 2 * MT>(ta, tile);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag(f, 2 * t), b[0], acc[t], 0, 0, 0);
+        }
+        const TrFrag f = tr_read<D, 2 * MT + 1>(ta, tile);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag(f, 2 * t), b[1], acc[t], 0, 0, 0);
+    }
+}
+
+// init + (tile rows 32 mt ..) . (resident rows)^T; roff: row_off() of this lane for mt
+template <int D>
+__device__ __forceinline__ f32x16 mfma_rows(const char* tile, int roff, const bf16x8 (&b)[D / 16], f32x16 init) {
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+        init = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(tile + (roff ^ (ks << 5))), b[ks], init, 0, 0, 0);
+    return init;
+}
+template <int D>
+__device__ __forceinline__ int row_off(int mt, int l31, int hi) {
+    const int r = mt * 32 + l31;
+    return r * 2 * D + ((hi ^ swz<D>(r)) << 4);
+}
+
+__device__ __forceinline__ f32x16 splat16(float v) {
+    f32x16 r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = v;
+    return r;
+}
+
+// maximum / sum of a value over the two half-waves that share a resident row
+__device__ __forceinline__ float half_max(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// Row of D outputs from accumulators [column 32 t + crow(r, hi)][row on the lane]: a half-wave exchange leaves 16
+// contiguous bytes in every lane.  All lanes take part; `on` guards the store.
+template <int D>
+__device__ __forceinline__ void store_row(__bf16* row, const f32x16 (&o)[D / 32], float mul, int hi, bool on) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            const unsigned ax = pack_bf16x2(o[t][4 * g] * mul, o[t][4 * g + 1] * mul);
+            const unsigned ay = pack_bf16x2(o[t][4 * g + 2] * mul, o[t][4 * g + 3] * mul);
+            const unsigned bx = pack_bf16x2(o[t][4 * g + 4] * mul, o[t][4 * g + 5] * mul);
+            const unsigned by = pack_bf16x2(o[t][4 * g + 6] * mul, o[t][4 * g + 7] * mul);
+            const auto sx = __builtin_amdgcn_permlane32_swap(ax, bx, false, false);
+            const auto sy = __builtin_amdgcn_permlane32_swap(ay, by, false, false);
+            if (on) *(u32x4*)(row + 32 * t + 8 * g + 8 * hi) = u32x4{sx[0], sy[0], sx[1], sy[1]};
+        }
+}
+
+// ---- which rows a block owns -------------------------------------------------------------------------------------------
+// The stretches of tokens are the sequences plus what lies before the first and behind the last.  Stretch e (0 .. n + 1)
+// starts at B(e) and gets block numbers from B(e) / BLK + e on: at least ceil(length / BLK) of them, so the grid
+// N / BLK + n + 2 is known without reading cu_seqlens, and a block finds its stretch by a 64-way search.  Offsets are
+// clamped into [0, N]: a bad cu_seqlens cannot lead outside the buffers.
+struct Span {
+    int64_t s0;
+    int len, first;  // rows of the stretch, first row of the block
+    bool dead;       // no sequence: outputs are zeros
+};
+__device__ __forceinline__ Span find_span(int b, const int* __restrict__ cu, int n, int N, int blk) {
+    const int lane = threadIdx.x & 63;
+    auto start = [&](int e) { return e <= 0 ? 0 : e >= n + 2 ? N : min(max(cu[e - 1], 0), N); };
+    int lo = 0, cnt = n + 2;
+    while (cnt > 1) {
+        const int step = (cnt + 63) >> 6;
+        const int k = lane * step;
+        const unsigned long long m = __ballot(k < cnt && start(lo + k) / blk + lo + k <= b);
+        const int w = m ? 63 - __builtin_clzll(m) : 0;
+        lo += w * step;
+        cnt = min(step, cnt - w * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    Span s;
+    const int a = start(lo), z = max(start(lo + 1), a);
+    s.s0 = a;
+    s.len = z - a;
+    const int64_t first = (int64_t)(b - a / blk - lo) * blk;
+    s.first = first < s.len ? (int)first : s.len;
+    s.dead = lo == 0 || lo == n + 1;
+    return s;
+}
+
+// Keys of tile kt that take part, one bit each.
+__device__ __forceinline__ unsigned char mask_byte(const unsigned char* mask, int64_t s0, int row, int len) {
+    return row < len ? (mask ? mask[s0 + row] : 1) : 0;
+}
+// Zero the rows of a landed tile whose bit is clear (a masked row may hold NaN or inf, and 0 times those is NaN).
+template <int D>
+__device__ __forceinline__ void zero_rows(char* tile, unsigned long long bits) {
+    const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
+    if (!((bits >> r) & 1))
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) *(u32x4*)(tile + r * 2 * D + part * (D / 2) + i * 16) = u32x4{0u, 0u, 0u, 0u};
+}
+
+// ---- forward -----------------------------------------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
+                                                                     float* __restrict__ lse, const int* __restrict__ cu,
+                                                                     int n_seg, const unsigned char* __restrict__ mask,
+                                                                     int N, int H, int group, int n_blk, int grid, float c) {
+    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_remap(blockIdx.x, grid);
+    const int head = id / n_blk;
+    const Span sp = find_span(id - head * n_blk, cu, n_seg, N, 128);
+    if (sp.first >= sp.len) return;
+    const int row = sp.first + wave * 32 + l31;
+    const bool on = row < sp.len;
+    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
+    __bf16* op = o.p + tok * o.tok + head * o.head;
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] = splat16(0.f);
+    if (sp.dead) {
+        store_row<D>(op, acc, 0.f, hi, on);
+        if (on && hi == 0) lse[(int64_t)head * N + tok] = -INFINITY;
+        return;
+    }
+    const __bf16* kb = k.p + sp.s0 * k.tok + (head / group) * k.head;
+    const __bf16* vb = v.p + sp.s0 * v.tok + (head / group) * v.head;
+    Stage<D> sk, sv;
+    sk.init(k.tok, wave, lane);
+    sv.init(v.tok, wave, lane);
+    const int nt = (sp.len + TR - 1) / TR;
+    auto stage = [&](int slot, int kt) {
+        char* base = smem + slot;
+        sk.go(base, kb + (int64_t)kt * TR * k.tok, sp.len - kt * TR, wave);
+        sv.go(base + TILE, vb + (int64_t)kt * TR * v.tok, sp.len - kt * TR, wave);
+    };
+    stage(0, 0);
+    unsigned char mb = mask_byte(mask, sp.s0, lane, sp.len);
+    bf16x8 qf[D / 16];
+    {
+        const __bf16* qp = q.p + tok * q.tok + head * q.head + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8*)(qp + ks * 16);
+    }
+    int koff[2];
+    koff[0] = row_off<D>(0, l31, hi);
+    koff[1] = row_off<D>(1, l31, hi);
+    TrAddr<D> ta;
+    ta.init(lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    float m = -INFINITY, l = 0.f;  // running maximum of q.k (before the scale), this half-wave's part of the row sum
+
+    auto tile = [&](auto masked, int cur, unsigned long long bits) {
+        constexpr bool MASKED = decltype(masked)::value;
+        f32x16 s[2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            s[mt] = mfma_rows<D>(smem + cur, koff[mt], qf, splat16(0.f));
+            if constexpr (MASKED) {
+                const unsigned b = (unsigned)(bits >> (32 * mt)) >> (4 * hi);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(b & (1u << crow(r, 0)))) s[mt][r] = -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[1][r]);
+        mx = half_max(mx);
+        // The reference point only follows a maximum that has outgrown it by 2^8 (any reference point gives the same
+        // quotient; fp32 sums and bf16 probabilities have the range).
+        if (__any((mx - m) * c > 8.f)) {
+            const float mn = fmaxf(m, mx);
+            const float a = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[t][r] *= a;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        bf16x8 p[2][2];
+        float ps = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[mt][r], c, -mc));
+                ps += e;
+                p[mt][r >> 3][r & 7] = (__bf16)e;  // 2^-9 relative, in the product with V only; the row sum keeps fp32
+            }
+        l += ps;
+        mfma_tr<D, 0>(acc, ta, lds0 + cur + TILE, p[0]);
+        mfma_tr<D, 1>(acc, ta, lds0 + cur + TILE, p[1]);
+    };
+    for (int kt = 0; kt < nt; ++kt) {
+        const int cur = (kt & 1) * SLOT, left = sp.len - kt * TR;
+        const unsigned long long bits = __ballot(mb != 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // tile kt has landed for every wave, and the other slot is read by none
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + 1 < nt) {
+            stage(SLOT - cur, kt + 1);
+            mb = mask_byte(mask, sp.s0, (kt + 1) * TR + lane, sp.len);
+        }
+        if (mask && bits != (left >= TR ? ~0ull : (1ull << left) - 1)) {  // uniform: every wave has the same bits
+            zero_rows<D>(smem + cur + TILE, bits);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+        }
+        if (bits == ~0ull) tile(std::false_type{}, cur, bits);
+        else if (bits) tile(std::true_type{}, cur, bits);
+    }
+    l = half_sum(l);
+    store_row<D>(op, acc, l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l), hi, on);  // no key: zeros; NaN stays
+    if (on && hi == 0) lse[(int64_t)head * N + tok] = l == 0.f ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * AG_LN2;
+}
+
+// ---- backward: dQ and delta --------------------------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dq_kernel(View dout, View q, View k, View v, View o,
+                                                                    const float* __restrict__ lse,
+                                                                    float* __restrict__ delta, OutView dq,
+                                                                    const int* __restrict__ cu, int n_seg,
+                                                                    const unsigned char* __restrict__ mask, int N, int H,
+                                                                    int group, int n_blk, int grid, float scale) {
+    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_remap(blockIdx.x, grid);
+    const int head = id / n_blk;
+    const Span sp = find_span(id - head * n_blk, cu, n_seg, N, 128);
+    if (sp.first >= sp.len) return;
+    const int row = sp.first + wave * 32 + l31;
+    const bool on = row < sp.len;
+    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
+    __bf16* op = dq.p + tok * dq.tok + head * dq.head;
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] = splat16(0.f);
+    if (sp.dead) {
+        store_row<D>(op, acc, 0.f, hi, on);
+        return;
+    }
+    const __bf16* kb = k.p + sp.s0 * k.tok + (head / group) * k.head;
+    const __bf16* vb = v.p + sp.s0 * v.tok + (head / group) * v.head;
+    Stage<D> sk, sv;
+    sk.init(k.tok, wave, lane);
+    sv.init(v.tok, wave, lane);
+    const int nt = (sp.len + TR - 1) / TR;
+    auto stage = [&](int slot, int kt) {
+        char* base = smem + slot;
+        sk.go(base, kb + (int64_t)kt * TR * k.tok, sp.len - kt * TR, wave);
+        sv.go(base + TILE, vb + (int64_t)kt * TR * v.tok, sp.len - kt * TR, wave);
+    };
+    stage(0, 0);
+    unsigned char mb = mask_byte(mask, sp.s0, lane, sp.len);
+    bf16x8 qf[D / 16], gf[D / 16];
+    float dl = 0.f;
+    {
+        const __bf16* qp = q.p + tok * q.tok + head * q.head + hi * 8;
+        const __bf16* gp = dout.p + tok * dout.tok + head * dout.head + hi * 8;
+        const __bf16* xp = o.p + tok * o.tok + head * o.head + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            qf[ks] = *(const bf16x8*)(qp + ks * 16);
+            gf[ks] = *(const bf16x8*)(gp + ks * 16);
+            const bf16x8 xf = *(const bf16x8*)(xp + ks * 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dl += (float)gf[ks][j] * (float)xf[j];
+        }
+    }
+    dl = half_sum(dl);
+    const float c = scale * AG_LOG2E;
+    const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;  // +inf for a row without keys: every key is masked there
+    if (on && hi == 0) delta[(int64_t)head * N + tok] = dl;
+    int koff[2];
+    koff[0] = row_off<D>(0, l31, hi);
+    koff[1] = row_off<D>(1, l31, hi);
+    TrAddr<D> ta;
+    ta.init(lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+
+    auto half = [&](auto masked, auto mt_, int cur, unsigned long long bits) {
+        constexpr bool MASKED = decltype(masked)::value;
+        constexpr int mt = decltype(mt_)::value;
+        const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, splat16(0.f));
+        const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], gf, splat16(0.f));
+        bf16x8 ds[2];
+        const unsigned b = (unsigned)(bits >> (32 * mt)) >> (4 * hi);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float e = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * (dp[r] - dl);
+            if constexpr (MASKED)
+                if (!(b & (1u << crow(r, 0)))) e = 0.f;
+            ds[r >> 3][r & 7] = (__bf16)e;  // 2^-9 relative, for the product with K
+        }
+        mfma_tr<D, mt>(acc, ta, lds0 + cur, ds);
+    };
+    for (int kt = 0; kt < nt; ++kt) {
+        const int cur = (kt & 1) * SLOT, left = sp.len - kt * TR;
+        const unsigned long long bits = __ballot(mb != 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + 1 < nt) {
+            stage(SLOT - cur, kt + 1);
+            mb = mask_byte(mask, sp.s0, (kt + 1) * TR + lane, sp.len);
+        }
+        if (mask && bits != (left >= TR ? ~0ull : (1ull << left) - 1)) {
+            zero_rows<D>(smem + cur, bits);
+            zero_rows<D>(smem + cur + TILE, bits);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+        }
+        if (bits == ~0ull) {
+            half(std::false_type{}, std::integral_constant<int, 0>{}, cur, bits);
+            half(std::false_type{}, std::integral_constant<int, 1>{}, cur, bits);
+        } else if (bits) {
+            half(std::true_type{}, std::integral_constant<int, 0>{}, cur, bits);
+            half(std::true_type{}, std::integral_constant<int, 1>{}, cur, bits);
+        }
+    }
+    store_row<D>(op, acc, scale, hi, on);
+}
+
+// ---- backward: dK and dV -----------------------------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dkdv_kernel(View dout, View q, View k, View v,
+                                                                      const float* __restrict__ lse,
+                                                                      const float* __restrict__ delta, OutView dk,
+                                                                      OutView dv, const int* __restrict__ cu, int n_seg,
+                                                                      const unsigned char* __restrict__ mask, int N, int G,
+                                                                      int group, int n_blk, int grid, float scale) {
+    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][TR];  // slot, (-lse log2 e, -delta), row of the tile
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_remap(blockIdx.x, grid);
+    const int kvh = id / n_blk;
+    const Span sp = find_span(id - kvh * n_blk, cu, n_seg, N, 128);
+    if (sp.first >= sp.len) return;
+    const int row = sp.first + wave * 32 + l31;
+    const bool on = row < sp.len;
+    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
+    __bf16* okp = dk.p + tok * dk.tok + kvh * dk.head;
+    __bf16* ovp = dv.p + tok * dv.tok + kvh * dv.head;
+    f32x16 ak[D / 32], av[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = splat16(0.f);
+    const bool live = on && !sp.dead && (!mask || mask[tok]);
+    if (!__syncthreads_or(live)) {  // no key of the block takes part
+        store_row<D>(okp, ak, 0.f, hi, on);
+        store_row<D>(ovp, av, 0.f, hi, on);
+        return;
+    }
+    // A key that takes no part has its own lane: its column is computed from zero rows and not used.
+    bf16x8 kf[D / 16], vf[D / 16];
+    {
+        const __bf16* kp = k.p + tok * k.tok + kvh * k.head + hi * 8;
+        const __bf16* vp = v.p + tok * v.tok + kvh * v.head + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            u32x4 a = u32x4{0u, 0u, 0u, 0u}, b = a;
+            if (live) {
+                a = *(const u32x4*)(kp + ks * 16);
+                b = *(const u32x4*)(vp + ks * 16);
+            }
+            kf[ks] = __builtin_bit_cast(bf16x8, a);
+            vf[ks] = __builtin_bit_cast(bf16x8, b);
+        }
+    }
+    Stage<D> sq, sg;
+    sq.init(q.tok, wave, lane);
+    sg.init(dout.tok, wave, lane);
+    const int nt = (sp.len + TR - 1) / TR;  // query tiles per head of the group
+    const int total = nt * group;
+    float next = 0.f;
+    auto stage = [&](int slot, int i) {
+        const int g = i / nt, qt = i - g * nt, left = sp.len - qt * TR;
+        const int head = kvh * group + g;
+        const int64_t t0 = sp.s0 + (int64_t)qt * TR;
+        char* base = smem + slot;
+        sq.go(base, q.p + t0 * q.tok + head * q.head, left, wave);
+        sg.go(base + TILE, dout.p + t0 * dout.tok + head * dout.head, left, wave);
+        if (wave < 2) {  // wave 0: lse, wave 1: delta.  Rows past the end get probability 2^-inf = 0
+            const float* src = (wave ? delta : lse) + (int64_t)head * N + t0;
+            const float x = lane < left ? src[lane] : (wave ? 0.f : INFINITY);
+            next = wave ? -x : -x * AG_LOG2E;
+        }
+    };
+    stage(0, 0);
+    int koff[2];
+    koff[0] = row_off<D>(0, l31, hi);
+    koff[1] = row_off<D>(1, l31, hi);
+    TrAddr<D> ta;
+    ta.init(lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    const float c = scale * AG_LOG2E;
+
+    auto half = [&](auto mt_, int cur, const float* st) {
+        constexpr int mt = decltype(mt_)::value;
+        f32x16 nl, nd;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 a = *(const f32x4*)(st + 32 * mt + 8 * g + 4 * hi), b = *(const f32x4*)(st + TR + 32 * mt + 8 * g + 4 * hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { nl[4 * g + e] = a[e]; nd[4 * g + e] = b[e]; }
+        }
+        const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], kf, splat16(0.f));
+        const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], vf, nd);  // dO V^T - delta
+        bf16x8 p[2], ds[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl[r]));
+            p[r >> 3][r & 7] = (__bf16)e;  // 2^-9 relative, for the products with dO and Q
+            ds[r >> 3][r & 7] = (__bf16)(e * dp[r]);
+        }
+        mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
+        mfma_tr<D, mt>(ak, ta, lds0 + cur, ds);
+    };
+    for (int i = 0; i < total; ++i) {
+        const int cur = (i & 1) * SLOT;
+        if (wave < 2) stat[i & 1][wave][lane] = next;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 < total) stage(SLOT - cur, i + 1);
+        half(std::integral_constant<int, 0>{}, cur, &stat[i & 1][0][0]);
+        half(std::integral_constant<int, 1>{}, cur, &stat[i & 1][0][0]);
+    }
+    if (!live) {
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = splat16(0.f);
+    }
+    store_row<D>(okp, ak, scale, hi, on);
+    store_row<D>(ovp, av, 1.f, hi, on);
+}
+
+bool ag_strides(const void* p, const int64_t* st, int D) {
+    // 16-byte rows; a tile's offsets (64 rows) stay inside the 31 bits of a buffer descriptor
+    return ((uintptr_t)p & 15) == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[0] >= D && st[1] >= 0 && st[0] < (1 << 23);
+}
+
+int ag_check(const char* who, const int32_t* cu, int n_seg, int N, int H, int G, int D, float scale) {
+    if (D != 64 && D != 128) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: head dim %d (64 or 128)", who, D);
+    if (N < 0 || N > (1 << 30) || n_seg < 0 || H <= 0 || G <= 0 || H % G) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: n_tokens=%d, n_segments=%d, heads=%d, kv heads=%d", who, N, n_seg, H, G);
+    if (!(scale > 0.f && scale < 1e30f)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: scale must be positive and finite", who);
+    if (N > 0 && !cu) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (((long long)N / 128 + n_seg + 2) * H > 0x7fffffffLL) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: grid too large", who);
+    return ESMK_OK;
+}
+
+}  // namespace
+
+extern "C" int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                                    const int64_t* strides, const int32_t* cu_seqlens, int n_segments,
+                                    const uint8_t* key_mask, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                    float scale, esmk_stream_t stream) {
+    if (int rc = ag_check("esmk_attn_varlen_fwd", cu_seqlens, n_segments, n_tokens, n_heads, n_kv_heads, head_dim, scale)) return rc;
+    if (n_tokens == 0) return ESMK_OK;
+    if (!q || !k || !v || !out || !lse || !strides) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_fwd: null pointer");
+    const void* ps[4] = {q, k, v, out};
+    for (int i = 0; i < 4; ++i)
+        if (!ag_strides(ps[i], strides + 2 * i, head_dim))
+            ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_fwd: tensor %d: address and strides must be multiples of 16 bytes, token stride >= head_dim", i);
+    const View vq{(const __bf16*)q, strides[0], strides[1]}, vk{(const __bf16*)k, strides[2], strides[3]}, vv{(const __bf16*)v, strides[4], strides[5]};
+    const OutView vo{(__bf16*)out, strides[6], strides[7]};
+    const int n_blk = n_tokens / 128 + n_segments + 2, grid = n_blk * n_heads, group = n_heads / n_kv_heads;
+    auto* kern = head_dim == 64 ? attn_fwd_lse_kernel<64> : attn_fwd_lse_kernel<128>;
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(AG_WAVES * 64), 0, (hipStream_t)stream, vq, vk, vv, vo, lse, cu_seqlens, n_segments,
+                       key_mask, n_tokens, n_heads, group, n_blk, grid, scale * AG_LOG2E);
+    ESMK_CHECK_LAUNCH("esmk_attn_varlen_fwd");
+    return ESMK_OK;
+}
+
+extern "C" size_t esmk_attn_varlen_bwd_workspace_bytes(int n_tokens, int n_heads) {
+    return n_tokens <= 0 || n_heads <= 0 ? 0 : (size_t)n_tokens * n_heads * sizeof(float);
+}
+
+extern "C" int esmk_attn_varlen_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out,
+                                    const float* lse, void* dq, void* dk, void* dv, const int64_t* strides,
+                                    const int32_t* cu_seqlens, int n_segments, const uint8_t* key_mask, int n_tokens,
+                                    int n_heads, int n_kv_heads, int head_dim, float scale, void* workspace,
+                                    size_t workspace_bytes, esmk_stream_t stream) {
+    if (int rc = ag_check("esmk_attn_varlen_bwd", cu_seqlens, n_segments, n_tokens, n_heads, n_kv_heads, head_dim, scale)) return rc;
+    if (n_tokens == 0) return ESMK_OK;
+    if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv || !strides) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_bwd: null pointer");
+    const void* ps[8] = {dout, q, k, v, out, dq, dk, dv};
+    for (int i = 0; i < 8; ++i)
+        if (!ag_strides(ps[i], strides + 2 * i, head_dim))
+            ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_bwd: tensor %d: address and strides must be multiples of 16 bytes, token stride >= head_dim", i);
+    if (!workspace || workspace_bytes < esmk_attn_varlen_bwd_workspace_bytes(n_tokens, n_heads) || ((uintptr_t)workspace & 3))
+        ESMK_FAIL(ESMK_ERR_WORKSPACE, "esmk_attn_varlen_bwd: needs %zu workspace bytes", esmk_attn_varlen_bwd_workspace_bytes(n_tokens, n_heads));
+    auto in = [&](int i) { return View{(const __bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
+    auto ov = [&](int i) { return OutView{(__bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
+    const int n_blk = n_tokens / 128 + n_segments + 2, group = n_heads / n_kv_heads;
+    float* delta = (float*)workspace;
+    hipStream_t s = (hipStream_t)stream;
+    auto* kq = head_dim == 64 ? attn_bwd_dq_kernel<64> : attn_bwd_dq_kernel<128>;
+    hipLaunchKernelGGL(kq, dim3(n_blk * n_heads), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), in(4), lse, delta, ov(5),
+                       cu_seqlens, n_segments, key_mask, n_tokens, n_heads, group, n_blk, n_blk * n_heads, scale);
+    auto* kk = head_dim == 64 ? attn_bwd_dkdv_kernel<64> : attn_bwd_dkdv_kernel<128>;
+    hipLaunchKernelGGL(kk, dim3(n_blk * n_kv_heads), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), lse, delta, ov(6), ov(7),
+                       cu_seqlens, n_segments, key_mask, n_tokens, n_kv_heads, group, n_blk, n_blk * n_kv_heads, scale);
+    ESMK_CHECK_LAUNCH("esmk_attn_varlen_bwd");
+    return ESMK_OK;
+}

@@ -1,0 +1,316 @@
+// Preference loss of packed sequence pairs (paired log ratios against a frozen model), forward and backward.
+//
+//   l_s = sum of log softmax(z_t)[y_t] over the scored tokens of sequence s
+//   m_i = beta ((l_2i - ref_2i) - (l_2i+1 - ref_2i+1))
+//   L   = mean_i [(1 - eps) softplus(-m_i) + eps softplus(m_i) - alpha l_2i / max(1, scored_2i)]
+//   dL/dz_t = c_t (onehot(y_t) - softmax z_t),  c_t = dL/dl of its sequence, 0 where the token is not scored
+//
+// A token's softmax needs its row of logits alone, a row's gradient needs both sequences of its pair: so one pass over the
+// logits leaves (max, log-sum, log-probability) of every token, a workgroup per pair adds the log-probabilities (in 64
+// bits: a margin is a small difference of two long sums) and leaves c_t, and the backward pass reads the logits once more
+// and writes the gradient.  All three are bound by memory; sums run in a fixed order.
+#include "common.hpp"
+
+namespace {
+
+// token state: max, log of the sum of exp(z - max), log-probability of the target, c_t
+typedef f32x4 TokState;
+
+template <typename T> struct PlT;
+template <> struct PlT<float> { static constexpr int N = 4; };
+template <> struct PlT<__bf16> { static constexpr int N = 8; };
+
+__device__ __forceinline__ float pl_get(const float* p) { return *p; }
+__device__ __forceinline__ float pl_get(const __bf16* p) { return (float)*p; }
+__device__ __forceinline__ void pl_unpack(const float* p, float (&f)[4]) {
+    const f32x4 v = *(const f32x4*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = v[e];
+}
+__device__ __forceinline__ void pl_unpack(const __bf16* p, float (&f)[8]) {
+    const u32x4 v = *(const u32x4*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f[2 * e] = __uint_as_float(v[e] << 16);
+        f[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void pl_store(float* p, const float (&f)[4]) { *(f32x4*)p = f32x4{f[0], f[1], f[2], f[3]}; }
+__device__ __forceinline__ void pl_store(__bf16* p, const float (&f)[8]) {
+    *(u32x4*)p = u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+}
+
+constexpr float PL_LOG2E = 1.4426950408889634f, PL_LN2 = 0.6931471805599453f;
+
+// exp(x) for x <= 0 with the product x log2(e) carried in two parts: exp2 alone would lose |x| 2^-24 of the result
+__device__ __forceinline__ float pl_exp(float x) {
+    const float h = x * PL_LOG2E;
+    const float l = fmaf(x, PL_LOG2E, -h) + x * 1.9259629911e-8f;  // log2(e) - fp32(log2(e))
+    const float r = __builtin_amdgcn_exp2f(h);
+    return h < -3e38f ? 0.f : fmaf(r * PL_LN2, l, r);  // x = -inf makes l NaN; a NaN x stays one
+}
+
+// Rows start at any element: a row is covered by 16-byte pieces of memory; the first and the last may hold elements of
+// the neighbouring rows, and are read and written element by element.
+template <typename T>
+struct Row {
+    const T* base;  // 16-byte aligned, at or below the row's first element
+    int lead, n_pieces, V;
+    __device__ __forceinline__ Row(const T* z, int64_t row, int V_) : V(V_) {
+        const T* p = z + row * V_;
+        lead = (int)(((uintptr_t)p & 15) / sizeof(T));
+        base = p - lead;
+        n_pieces = (lead + V_ + PlT<T>::N - 1) / PlT<T>::N;
+    }
+    __device__ __forceinline__ int col(int piece) const { return piece * PlT<T>::N - lead; }
+    __device__ __forceinline__ bool whole(int c) const { return c >= 0 && c + PlT<T>::N <= V; }
+    __device__ __forceinline__ void load(int piece, float (&f)[PlT<T>::N], float fill) const {
+        const int c = col(piece);
+        if (whole(c)) {
+            pl_unpack(base + (int64_t)piece * PlT<T>::N, f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < PlT<T>::N; ++e)
+                f[e] = c + e >= 0 && c + e < V ? pl_get(base + (int64_t)piece * PlT<T>::N + e) : fill;
+        }
+    }
+};
+
+template <int LPR>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+template <int LPR>
+__device__ __forceinline__ float row_add(float v) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// LPR lanes per row
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void pref_token_kernel(const T* __restrict__ z, const int64_t* __restrict__ targets,
+                                                         TokState* __restrict__ tok, int N, int V) {
+    constexpr int E = PlT<T>::N, CH = 4;  // pieces in flight per lane
+    const int sub = threadIdx.x & (LPR - 1);
+    const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    if (row >= N) return;
+    const int64_t y = targets[row];
+    if (y < 0 || y >= V) {  // not scored: its logits are not looked at
+        if (sub == 0) tok[row] = TokState{0.f, 0.f, 0.f, 0.f};
+        return;
+    }
+    const Row<T> r(z, row, V);
+    float m = -INFINITY, l = 0.f;
+    for (int p0 = sub; p0 < r.n_pieces; p0 += LPR * CH) {
+        float f[CH][E];
+        float t = m;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            if (p0 + i * LPR < r.n_pieces) r.load(p0 + i * LPR, f[i], -INFINITY);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[i][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) t = fmaxf(t, f[i][e]);
+        const float base = t == -INFINITY ? 0.f : t;  // only -inf so far: exp(-inf) = 0, and not exp(-inf + inf)
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((f[i][e] - base) * PL_LOG2E);
+        l = l * __builtin_amdgcn_exp2f((m - base) * PL_LOG2E) + s;
+        m = t;
+    }
+    const float top = row_max<LPR>(m);
+    l = row_add<LPR>(l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * PL_LOG2E)));
+    if (sub == 0) {
+        const float ls = logf(l);  // no finite logit: log 0, and the row's loss is not finite, as the formula has it
+        tok[row] = TokState{top, ls, (pl_get(z + row * V + y) - top) - ls, 0.f};
+    }
+}
+
+// one workgroup per pair
+__global__ __launch_bounds__(256) void pref_pair_kernel(const int64_t* __restrict__ targets, TokState* __restrict__ tok,
+                                                        const int* __restrict__ cu, const float* __restrict__ ref, int N,
+                                                        int V, int P, double beta, double eps, double alpha,
+                                                        float* __restrict__ logps, double* __restrict__ pair_loss,
+                                                        float* __restrict__ loss) {
+    __shared__ double red[2][4];
+    __shared__ int cnt[4];
+    const int i = blockIdx.x, wave = threadIdx.x >> 6;
+    int lo[2], hi[2], scored = 0;
+    double l[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        lo[s] = min(max(cu[2 * i + s], 0), N);
+        hi[s] = min(max(cu[2 * i + s + 1], lo[s]), N);
+        double a = 0.0;
+        int n = 0;
+        for (int t = lo[s] + (int)threadIdx.x; t < hi[s]; t += 256) {
+            const int64_t y = targets[t];
+            if (y >= 0 && y < V) {
+                a += (double)tok[t][2];
+                ++n;
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o); n += __shfl_xor(n, o); }
+        if ((threadIdx.x & 63) == 0) {
+            red[s][wave] = a;
+            if (s == 0) cnt[wave] = n;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) l[s] = (red[s][0] + red[s][1]) + (red[s][2] + red[s][3]);
+    scored = max(1, cnt[0] + cnt[1] + cnt[2] + cnt[3]);
+    const double m = beta * ((l[0] - (double)ref[2 * i]) - (l[1] - (double)ref[2 * i + 1]));
+    const double t = exp(-fabs(m)), up = m >= 0.0 ? 1.0 / (1.0 + t) : t / (1.0 + t), down = m >= 0.0 ? t / (1.0 + t) : 1.0 / (1.0 + t);
+    const double lg = log1p(t), sp = fmax(m, 0.0) + lg, sn = fmax(-m, 0.0) + lg;
+    // a term whose weight is zero is left out: 0 x inf would be NaN
+    double L = eps != 1.0 ? (1.0 - eps) * sn : 0.0;
+    if (eps != 0.0) L += eps * sp;
+    if (alpha != 0.0) L -= alpha * l[0] / scored;
+    const double gm = beta * (eps * up - (1.0 - eps) * down) / P;
+    const float c[2] = {(float)(gm - alpha / scored / P), (float)-gm};
+    if (threadIdx.x == 0) {
+        logps[2 * i] = (float)l[0];
+        logps[2 * i + 1] = (float)l[1];
+        if (P == 1) *loss = (float)L;
+        else pair_loss[i] = L;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+        for (int k = lo[s] + (int)threadIdx.x; k < hi[s]; k += 256) {
+            const int64_t y = targets[k];
+            if (y >= 0 && y < V) tok[k][3] = c[s];
+        }
+}
+
+__global__ __launch_bounds__(256) void pref_mean_kernel(const double* __restrict__ pair_loss, int P, float* __restrict__ loss) {
+    __shared__ double red[4];
+    double a = 0.0;
+    for (int i = threadIdx.x; i < P; i += 256) a += pair_loss[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) *loss = (float)(((red[0] + red[1]) + (red[2] + red[3])) / P);
+}
+
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void pref_grad_kernel(const T* __restrict__ z, const int64_t* __restrict__ targets,
+                                                        const TokState* __restrict__ tok, const float* __restrict__ grad,
+                                                        T* __restrict__ dz, int N, int V) {
+    constexpr int E = PlT<T>::N;
+    const int sub = threadIdx.x & (LPR - 1);
+    const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    if (row >= N) return;
+    const TokState st = tok[row];
+    const int64_t y = targets[row];
+    const bool on = st[3] != 0.f;  // 0: not scored, or behind the last sequence
+    const float c = on ? (grad ? st[3] * *grad : st[3]) : 0.f;
+    const Row<T> r(z, row, V);
+    T* out = dz + row * V - r.lead;
+    for (int p = sub; p < r.n_pieces; p += LPR) {
+        float f[E], o[E];
+        const int col = r.col(p);
+        if (on) {
+            r.load(p, f, 0.f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float q = pl_exp((f[e] - st[0]) - st[1]);
+                o[e] = c * ((col + e == (int)y ? 1.f : 0.f) - q);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = 0.f;
+        }
+        T* q = out + (int64_t)p * E;
+        if (r.whole(col)) {
+            pl_store(q, o);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (col + e >= 0 && col + e < V) q[e] = (T)o[e];
+        }
+    }
+}
+
+// 16 lanes per row up to 256 entries (the 64-entry vocabulary is one 16-byte piece per lane), a wave above.
+template <typename F>
+void pl_dispatch(int V, F f) {
+    if (V <= 256) f(std::integral_constant<int, 16>{});
+    else f(std::integral_constant<int, 64>{});
+}
+
+template <typename T>
+void pl_token(const void* z, const int64_t* y, TokState* tok, int N, int V, hipStream_t s) {
+    pl_dispatch(V, [&](auto lpr) {
+        constexpr int LPR = decltype(lpr)::value;
+        hipLaunchKernelGGL((pref_token_kernel<T, LPR>), dim3((N + 256 / LPR - 1) / (256 / LPR)), dim3(256), 0, s, (const T*)z, y, tok, N, V);
+    });
+}
+template <typename T>
+void pl_grad(const void* z, const int64_t* y, const TokState* tok, const float* g, void* dz, int N, int V, hipStream_t s) {
+    pl_dispatch(V, [&](auto lpr) {
+        constexpr int LPR = decltype(lpr)::value;
+        hipLaunchKernelGGL((pref_grad_kernel<T, LPR>), dim3((N + 256 / LPR - 1) / (256 / LPR)), dim3(256), 0, s, (const T*)z, y, tok, g, (T*)dz, N, V);
+    });
+}
+
+int pl_check(const char* who, const void* z, int dtype, const void* targets, const void* saved, int N, int V) {
+    if (N < 0 || V <= 0 || V > (1 << 30)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: N=%d, V=%d", who, N, V);
+    if (dtype != ESMK_F32 && dtype != ESMK_BF16) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: bad dtype %d", who, dtype);
+    if (N > 0 && (!z || !targets || !saved)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (((uintptr_t)z | (uintptr_t)saved) & 15) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: logits and saved must be 16-byte aligned", who);
+    return ESMK_OK;
+}
+
+}  // namespace
+
+extern "C" size_t esmk_pref_loss_saved_bytes(int N, int n_pairs) {
+    return N < 0 || n_pairs < 0 ? 0 : (size_t)N * sizeof(TokState) + (size_t)n_pairs * sizeof(double);
+}
+
+extern "C" int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* targets, const int32_t* cu_seqlens,
+                                  int n_pairs, const float* ref_logps, double beta, double label_smoothing, double nll_weight,
+                                  int N, int V, void* saved, size_t saved_bytes, float* logps, float* loss,
+                                  esmk_stream_t stream) {
+    if (int rc = pl_check("esmk_pref_loss_fwd", logits, dtype, targets, saved, N, V)) return rc;
+    if (n_pairs <= 0) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: n_pairs=%d", n_pairs);
+    if (!cu_seqlens || !ref_logps || !logps || !loss || !saved) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: null pointer");
+    if (!(label_smoothing >= 0.0 && label_smoothing <= 1.0)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: label_smoothing outside [0, 1]");
+    if (saved_bytes < esmk_pref_loss_saved_bytes(N, n_pairs))
+        ESMK_FAIL(ESMK_ERR_WORKSPACE, "esmk_pref_loss_fwd: saved needs %zu bytes", esmk_pref_loss_saved_bytes(N, n_pairs));
+    hipStream_t s = (hipStream_t)stream;
+    TokState* tok = (TokState*)saved;
+    double* pair_loss = (double*)(tok + N);
+    if (N > 0) {
+        if (dtype == ESMK_F32) pl_token<float>(logits, targets, tok, N, V, s);
+        else pl_token<__bf16>(logits, targets, tok, N, V, s);
+    }
+    hipLaunchKernelGGL(pref_pair_kernel, dim3(n_pairs), dim3(256), 0, s, targets, tok, cu_seqlens, ref_logps, N, V, n_pairs,
+                       beta, label_smoothing, nll_weight, logps, pair_loss, loss);
+    if (n_pairs > 1) hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(256), 0, s, pair_loss, n_pairs, loss);
+    ESMK_CHECK_LAUNCH("esmk_pref_loss_fwd");
+    return ESMK_OK;
+}
+
+extern "C" int esmk_pref_loss_bwd(const void* logits, int dtype, const int64_t* targets, const void* saved,
+                                  const float* grad_loss, void* dlogits, int N, int V, esmk_stream_t stream) {
+    if (int rc = pl_check("esmk_pref_loss_bwd", logits, dtype, targets, saved, N, V)) return rc;
+    if (N == 0) return ESMK_OK;
+    if (!dlogits || ((uintptr_t)dlogits & 15)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_bwd: dlogits must be 16-byte aligned");
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == ESMK_F32) pl_grad<float>(logits, targets, (const TokState*)saved, grad_loss, dlogits, N, V, s);
+    else pl_grad<__bf16>(logits, targets, (const TokState*)saved, grad_loss, dlogits, N, V, s);
+    ESMK_CHECK_LAUNCH("esmk_pref_loss_bwd");
+    return ESMK_OK;
+}

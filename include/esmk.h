@@ -245,6 +245,64 @@ int esmk_attn_l64_d128(const void* qkv_bf16, void* ctx_bf16, const float* rope_c
                        int n_sequences, int d, int n_heads, esmk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Training: LayerNorm, block-diagonal attention and a paired preference loss, each with its gradient.  The reference
+ * gets these gradients from torch's autograd over the modules named at the forward entry points above
+ * (esm/layers/attention.py:26-33,65-78; esm/layers/blocks.py:31); the loss has no counterpart there.
+ * Every sum runs in a fixed order: the same inputs give the same bits.  Nothing is kept between calls.
+ * ------------------------------------------------------------------------------------------ */
+
+/* y [M, d] = LayerNorm(x) and stats f32 [M][2] = (mean, 1/sqrt(var + eps)) of every row.  x, y: dtype (F32 or BF16);
+ * x rows are ldx >= d elements apart, y rows d.  gamma f32 [d]; beta f32 [d] or NULL.  1 <= d <= 12288, any address that
+ * suits the type.  stats 8-byte aligned. */
+int esmk_layernorm_fwd(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, void* y, float* stats,
+                       int M, int d, float eps, esmk_stream_t stream);
+/* dx [M, d] (dtype, dense rows); dgamma, dbeta f32 [d], overwritten (either may be NULL: not wanted).  dy, x: dtype, rows
+ * lddy / ldx >= d elements apart; stats from esmk_layernorm_fwd.  workspace: esmk_layernorm_bwd_workspace_bytes (needed
+ * only where dgamma or dbeta is).  M = 0 sets dgamma and dbeta to zero. */
+size_t esmk_layernorm_bwd_workspace_bytes(int M, int d);
+int esmk_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int dtype, const float* gamma,
+                       const float* stats, void* dx, float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes,
+                       int M, int d, esmk_stream_t stream);
+
+/* out = softmax(scale q k^T) v inside every sequence cu_seqlens[s] .. cu_seqlens[s + 1] (int32 [n_segments + 1], device,
+ * non-decreasing, within [0, n_tokens]: values outside are clamped), and lse f32 [n_heads][n_tokens], the natural log of
+ * the sum of exponentials.  Tensors bf16 [token][head][head_dim], head_dim 64 or 128, head_dim dense; strides (host,
+ * elements, two per tensor: token, head) in the order of the arguments, each a multiple of 8, addresses 16-byte aligned,
+ * token strides >= head_dim and below 2^23.  k and v have n_kv_heads heads, which divides n_heads: query head h reads key
+ * head h / (n_heads / n_kv_heads).  key_mask uint8 [n_tokens] or NULL: keys whose byte is 0 take no part, whatever they hold
+ * (the token's own query does).  A query without any key gets out = 0, lse = -inf; tokens in no sequence likewise.
+ * scale > 0; n_tokens <= 2^30. */
+int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides,
+                         const int32_t* cu_seqlens, int n_segments, const uint8_t* key_mask, int n_tokens, int n_heads,
+                         int n_kv_heads, int head_dim, float scale, esmk_stream_t stream);
+/* Gradients of the same with respect to q, k and v, from out and lse of esmk_attn_varlen_fwd on the same inputs.  strides:
+ * 16 values for dout, q, k, v, out, dq, dk, dv.  dk and dv are summed over the query heads that share a key head.  Masked
+ * keys, queries without a key and tokens in no sequence get zeros.  workspace: esmk_attn_varlen_bwd_workspace_bytes, owned by
+ * this call while it runs. */
+size_t esmk_attn_varlen_bwd_workspace_bytes(int n_tokens, int n_heads);
+int esmk_attn_varlen_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                         void* dq, void* dk, void* dv, const int64_t* strides, const int32_t* cu_seqlens, int n_segments,
+                         const uint8_t* key_mask, int n_tokens, int n_heads, int n_kv_heads, int head_dim, float scale,
+                         void* workspace, size_t workspace_bytes, esmk_stream_t stream);
+
+/* Preference loss over n_pairs >= 1 pairs of packed sequences: sequence 2i is the preferred one of pair i, 2i + 1 the other.
+ *   logps[s] = sum of log softmax(logits[t])[targets[t]] over the scored tokens of sequence s
+ *   m_i      = beta ((logps[2i] - ref_logps[2i]) - (logps[2i+1] - ref_logps[2i+1]))
+ *   loss     = mean_i [(1 - e) softplus(-m_i) + e softplus(m_i) - nll_weight logps[2i] / max(1, scored tokens of 2i)]
+ * with e = label_smoothing in [0, 1].  A token is scored if 0 <= targets[t] < V; other tokens, and tokens behind the last
+ * sequence, are skipped whatever their logits hold, and get a zero gradient.  logits [N, V] dense, F32 or BF16; targets
+ * int64 [N]; cu_seqlens int32 [2 n_pairs + 1] (device; clamped as above); ref_logps, logps f32 [2 n_pairs]; loss f32 [1].
+ * saved: esmk_pref_loss_saved_bytes, 16-byte aligned, for the backward call. */
+size_t esmk_pref_loss_saved_bytes(int N, int n_pairs);
+int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* targets, const int32_t* cu_seqlens, int n_pairs,
+                       const float* ref_logps, double beta, double label_smoothing, double nll_weight, int N, int V,
+                       void* saved, size_t saved_bytes, float* logps, float* loss, esmk_stream_t stream);
+/* dlogits [N, V] (dtype) = grad_loss times the loss's gradient; grad_loss f32 [1] on the device, NULL = 1.  logits and
+ * dlogits 16-byte aligned. */
+int esmk_pref_loss_bwd(const void* logits, int dtype, const int64_t* targets, const void* saved, const float* grad_loss,
+                       void* dlogits, int N, int V, esmk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Embedding gather: out f32 [M, d] = table[tokens].   Replaces nn.Embedding (esmc.py:63,137).
  * ------------------------------------------------------------------------------------------ */
 int esmk_embed(const int64_t* tokens, const float* table, int vocab, float* out, int M, int d,

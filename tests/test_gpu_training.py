@@ -1,0 +1,597 @@
+"""Training operators (esm_amd.training) against plain 64-bit computations of their formulas.
+
+Tolerances are bounds, element by element, derived from where the kernels round: u = 2^-24 for fp32 arithmetic,
+r = eps / 2 of the output type (2^-8 for bf16) for every rounding to it.  Each test states its bound where it forms it."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+R = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def T():
+    from esm_amd import training
+    return training
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def within(got, want, tol, what):
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got.double()).all(), f"{what}: not finite"
+    over = (got.double() - want).abs() - tol
+    assert (over <= 0).all(), f"{what}: {over.max().item():.3e} over the bound, {int((over > 0).sum())} of {over.numel()}"
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+
+def norm_oracle(x, w, b, dy, eps=1e-5):
+    """64-bit (y, dx, dw, db) and their bounds for output type x.dtype."""
+    r = R[x.dtype]
+    x, w, dy = x.double(), w.double(), dy.double()
+    b = torch.zeros_like(w) if b is None else b.double()
+    d = x.shape[-1]
+    mu = x.mean(-1, keepdim=True)
+    rs = 1 / ((x - mu).pow(2).mean(-1, keepdim=True) + eps).sqrt()
+    h = (x - mu) * rs
+    y = h * w + b
+    g = dy * w
+    c1, c2 = g.mean(-1, keepdim=True), (g * h).mean(-1, keepdim=True)
+    dx = rs * (g - c1 - h * c2)
+    # A row sum is at most 24 additions in a lane, 6 between lanes, 8 between waves: 40 u of the mean of the magnitudes.
+    # xc = x - mean: 41 u (|x| + mean|x|); rstd: relative 60 u plus the effect of xc; h: both.
+    ax = x.abs()
+    exc = 42 * U * (ax + ax.mean(-1, keepdim=True))
+    ers = 64 * U + 2 * (exc * (x - mu).abs()).mean(-1, keepdim=True) * rs * rs  # relative
+    eh = exc * rs + h.abs() * ers
+    ty = r * y.abs() + (1 + r) * (eh * w.abs() + 4 * U * (h * w).abs() + U * y.abs())
+    ec1 = 44 * U * g.abs().mean(-1, keepdim=True)
+    ec2 = ((eh + 44 * U * h.abs()) * g.abs()).mean(-1, keepdim=True)
+    inner = g.abs() + c1.abs() + (h * c2).abs()
+    ti = 4 * U * inner + ec1 + eh * c2.abs() + h.abs() * ec2
+    tdx = r * dx.abs() + (1 + r) * rs * (ti + inner * ers)
+    # columns: a lane adds its rows, then 3 row slots, 16 partials and 32 groups: below M + 64 additions
+    M = x.reshape(-1, d).shape[0]
+    n = min(M, M // 512 + 8) + 64
+    cols = lambda t: t.reshape(-1, d).sum(0)
+    dw, db = cols(dy * h), cols(dy)
+    tdw = cols(dy.abs() * eh) + n * U * cols((dy * h).abs())
+    tdb = n * U * cols(dy.abs())
+    return (y, dx, dw, db), (ty, tdx, tdw, tdb)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d", [(1, 1), (2, 3), (5, 64), (17, 65), (66, 960), (301, 1152), (130, 1281), (1030, 512),
+                                    (37, 2560), (33, 1537), (9, 4097), (7, 6145), (3, 12288), (4099, 33)])
+def test_layer_norm(rows, d, dtype):
+    g = gen(rows * 31 + d)
+    x = (randn(g, rows, d) * 2 + 0.5).to(dtype)
+    w, b, dy = 1 + 0.2 * randn(g, d), 0.3 * randn(g, d), randn(g, rows, d).to(dtype)
+    for bias in (None, b):
+        y, stats = T().layer_norm_forward(x, w, bias)
+        dx, dw, db = T().layer_norm_backward(dy, x, w, stats, bias=bias is not None)
+        assert y.dtype == dx.dtype == dtype and dw.dtype == torch.float32 and (db is None) == (bias is None)
+        want, tol = norm_oracle(x, w, bias, dy)
+        for got, a, t, n in zip((y, dx, dw, db), want, tol, ("y", "dx", "dw", "db")):
+            if got is not None:
+                within(got, a, t, n)
+
+
+def test_layer_norm_strides_ranks_and_parameter_types():
+    g = gen(5)
+    wide = randn(g, 70, 3 * 192).bfloat16()
+    w, b = 1 + 0.1 * randn(g, 192), 0.1 * randn(g, 192)
+    dyw = randn(g, 70, 2 * 192).bfloat16()
+    for x, dy in ((wide[:, 192:384], dyw[:, :192]), (wide[:, 1:193], dyw[:, 3:195]), (wide[::2, :192], dyw[::2, :192]),
+                  (wide[:, :192].t().contiguous().t(), dyw[:, :192]), (wide[:1, :192].expand(70, 192), dyw[:, :192])):
+        y, st = T().layer_norm_forward(x, w, b)
+        got = (y,) + T().layer_norm_backward(dy, x, w, st)
+        y2, st2 = T().layer_norm_forward(x.contiguous(), w, b)
+        for p, q in zip(got, (y2,) + T().layer_norm_backward(dy.contiguous(), x.contiguous(), w, st2)):
+            want, tol = norm_oracle(x, w, b, dy)
+            assert p.shape == q.shape
+        for p, a, t in zip(got, want, tol):
+            within(p, a, t, "strided")
+    x3 = wide[:, :192].reshape(2, 35, 192)
+    assert torch.equal(T().layer_norm_forward(x3, w, b)[0], T().layer_norm_forward(x3.reshape(70, 192), w, b)[0].view(2, 35, 192))
+    x1 = wide[0, :192]
+    assert T().layer_norm_forward(x1, w)[0].shape == (192,)
+    # parameters in bf16 count as the values they hold
+    assert torch.equal(T().layer_norm_forward(x1, w.bfloat16())[0], T().layer_norm_forward(x1, w.bfloat16().float())[0])
+
+
+def test_layer_norm_no_rows_gives_zero_parameter_gradients():
+    x, w = torch.empty(0, 96, device="cuda"), torch.ones(96, device="cuda")
+    y, st = T().layer_norm_forward(x, w)
+    dx, dw, db = T().layer_norm_backward(torch.empty_like(x), x, w, st)
+    assert y.shape == dx.shape == (0, 96) and not dw.any() and not db.any()
+
+
+def test_layer_norm_far_rows():
+    """Row offsets past 2^32 bytes."""
+    big = torch.empty(300 * 2 ** 23, dtype=torch.bfloat16, device="cuda")
+    x = big.as_strided((300, 64), (2 ** 23, 1))
+    g = gen(3)
+    x.copy_(randn(g, 300, 64))
+    w, dy = 1 + 0.1 * randn(g, 64), randn(g, 300, 64).bfloat16()
+    y, st = T().layer_norm_forward(x, w)
+    got = (y,) + T().layer_norm_backward(dy, x, w, st)
+    xc = x.contiguous()
+    y2, st2 = T().layer_norm_forward(xc, w)
+    for a, b in zip(got, (y2,) + T().layer_norm_backward(dy, xc, w, st2)):
+        assert torch.equal(a, b)
+
+
+def test_layer_norm_autograd_and_differences():
+    g = gen(11)
+    x, w, b = randn(g, 21, 130), 1 + 0.2 * randn(g, 130), 0.2 * randn(g, 130)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    probe = randn(g, 21, 130)
+    (T().layer_norm(*leaves) * probe).sum().backward()
+    want, tol = norm_oracle(x, w, b, probe)
+    for t, a, e in zip(leaves, want[1:], tol[1:]):
+        within(t.grad, a, e, "autograd")
+    # central differences of the 64-bit formula along a random direction; its own error is below 1e-8 of the slope's terms
+    f = lambda x, w, b: (norm_oracle(x, w, b, probe.double())[0][0] * probe.double()).sum().item()
+    for i, t in enumerate((x, w, b)):
+        v = randn(g, *t.shape).double()
+        at = lambda s: f(*[(u.double() + s * v if j == i else u.double()) for j, u in enumerate((x, w, b))])
+        R[torch.float64] = 0.0
+        slope = (at(1e-4) - at(-1e-4)) / 2e-4
+        bound = (tol[1 + i] * v.abs()).sum().item() + 1e-6 * (want[1 + i].abs() * v.abs()).sum().item()
+        assert abs((leaves[i].grad.double() * v).sum().item() - slope) <= bound
+    # a frozen weight asks for no reduction; a broadcast input's gradient is summed
+    row = randn(g, 1, 130).requires_grad_()
+    T().layer_norm(row.expand(21, 130), w, b).sum().backward()
+    assert row.grad.shape == (1, 130)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+def attention_oracle(q, k, v, cu, scale, mask, dout):
+    """64-bit (out, lse, dq, dk, dv) and bounds.  Where the kernels round: P to bf16 before P V and P^T dO (r), dS to bf16
+    before dS K and dS^T Q (r), outputs (r); delta uses the rounded out.  fp32: a score has D products (D u of their
+    magnitudes) and moves P by that, relatively; sums over keys or queries L u."""
+    r = R[torch.bfloat16]
+    N, H, D = q.shape
+    G = k.shape[1]
+    q, k, v, dout = (t.double() for t in (q, k, v, dout))
+    z = lambda *s: torch.zeros(*s, dtype=torch.float64, device=q.device)
+    o, dq, dk, dv = z(N, H, D), z(N, H, D), z(N, G, D), z(N, G, D)
+    to, tdq, tdk, tdv = z(N, H, D), z(N, H, D), z(N, G, D), z(N, G, D)
+    lse, tl = torch.full((H, N), -math.inf, dtype=torch.float64, device=q.device), z(H, N)
+    for a, e in zip(cu, cu[1:]):
+        keys = torch.arange(a, e, device=q.device)
+        if mask is not None:
+            keys = keys[mask[a:e].bool()]
+        L = e - a
+        if len(keys) == 0:
+            continue
+        for h in range(H):
+            Q, K, V, dO = q[a:e, h], k[keys, h // (H // G)], v[keys, h // (H // G)], dout[a:e, h]
+            S = Q @ K.t() * scale
+            ls = torch.logsumexp(S, -1, keepdim=True)
+            P = (S - ls).exp()
+            O = P @ V
+            eS = (D + 8) * U * scale * (Q.abs() @ K.abs().t()) + 4 * U * (S.abs() + ls.abs())  # abs, both S and S - lse
+            eP = 2 * eS.amax(-1, keepdim=True) + (L + 32) * U                                  # rel. of P
+            A = P @ V.abs()
+            tO = (r + eP) * A * (1 + r) + r * O.abs() + eP * O.abs()
+            dP = dO @ V.t()
+            dl = (dO * O).sum(-1, keepdim=True)
+            dS = P * (dP - dl)
+            eDl = (dO.abs() * tO).sum(-1, keepdim=True) + (D + 8) * U * (dO * O).abs().sum(-1, keepdim=True)
+            eDP = (D + 8) * U * (dO.abs() @ V.abs().t())
+            eds = P * (eDl + eDP + eP * (dP - dl).abs()) * (1 + r) + r * dS.abs()              # abs, of the rounded dS
+            n = (L + 32) * U
+            o[a:e, h], to[a:e, h] = O, tO
+            lse[h, a:e] = ls[:, 0]
+            tl[h, a:e] = eS.amax(-1) + (L + 32) * U + 4 * U * ls[:, 0].abs()
+            dq[a:e, h] = scale * dS @ K
+            tdq[a:e, h] = scale * ((eds + n * dS.abs()) @ K.abs())
+            dk[keys, h // (H // G)] += scale * dS.t() @ Q
+            tdk[keys, h // (H // G)] += scale * ((eds + n * dS.abs()).t() @ Q.abs())
+            dv[keys, h // (H // G)] += P.t() @ dO
+            tdv[keys, h // (H // G)] += ((r + eP + n) * P).t() @ dO.abs()
+    tdq, tdk, tdv = (t * (1 + r) + r * x.abs() + 4 * U * x.abs() for t, x in ((tdq, dq), (tdk, dk), (tdv, dv)))
+    return (o, lse, dq, dk, dv), (to, tl, tdq, tdk, tdv)
+
+
+def attention_inputs(seed, lens, H, G, D, tail=0, lead=0, q_gain=1.5):
+    g = gen(seed)
+    cu = [lead]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    N = cu[-1] + tail
+    qkv = randn(g, N, H + 2 * G, D)
+    qkv[:, :H] *= q_gain
+    qkv = qkv.bfloat16()
+    return qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:], cu, torch.tensor(cu, dtype=torch.int32, device="cuda"), randn(g, N, H, D).bfloat16(), g
+
+
+def attention_all(q, k, v, cu, dout, scale=None, mask=None):
+    out, lse = T().attention_varlen_forward(q, k, v, cu, scale, mask)
+    return (out, lse) + T().attention_varlen_backward(dout, q, k, v, out, lse, cu, scale, mask)
+
+
+def check_attention(q, k, v, cu, cut, dout, scale=None, mask=None):
+    got = attention_all(q, k, v, cut, dout, scale, mask)
+    want, tol = attention_oracle(q, k, v, cu, scale or q.shape[2] ** -0.5, mask, dout)
+    none = want[1] == -math.inf
+    assert torch.equal(got[1] == -math.inf, none)
+    lse = got[1].masked_fill(none, 0.0)
+    want = (want[0], want[1].masked_fill(none, 0.0)) + want[2:]
+    for a, b, t, n in zip((got[0], lse) + got[2:], want, tol, ("out", "lse", "dq", "dk", "dv")):
+        within(a, b, t, n)
+    return got
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,G,tail", [([1], 1, 1, 0), ([2, 1, 3], 2, 1, 0), ([0, 5, 0], 2, 2, 3), ([64], 1, 1, 0),
+                                           ([63, 65], 2, 2, 0), ([128, 129, 127], 3, 1, 9), ([200, 1, 77, 300], 4, 2, 0),
+                                           ([1100], 2, 2, 1), ([31] * 70, 1, 1, 5)])
+def test_attention(lens, H, G, tail, D):
+    q, k, v, cu, cut, dout, _ = attention_inputs(len(lens) * 7 + D, lens, H, G, D, tail)
+    check_attention(q, k, v, cu, cut, dout)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_key_mask(D):
+    """Scattered masked keys, a tile without any key, a sequence without any key, one key left."""
+    q, k, v, cu, cut, dout, g = attention_inputs(3 + D, [150, 40, 260, 90], 4, 2, D, tail=6, lead=5)
+    mask = torch.rand(len(q), generator=g, device="cuda") > 0.3
+    mask[cu[1]:cu[2]] = False
+    mask[cu[2] + 64:cu[2] + 128] = False
+    mask[cu[3]:cu[4]] = False
+    mask[cu[3] + 70] = True
+    for m in (mask, mask.to(torch.uint8)):
+        got = check_attention(q, k, v, cu, cut, dout, mask=m)
+    assert not got[0][cu[1]:cu[2]].any() and not got[2][cu[1]:cu[2]].any()
+    assert not got[0][:5].any() and not got[0][cu[-1]:].any() and not got[3][~mask].any() and not got[4][~mask].any()
+    # what masked keys and tokens in no sequence hold does not matter, NaN and inf included
+    k2, v2, d2, q2 = k.clone(), v.clone(), dout.clone(), q.clone()
+    k2[~mask], v2[~mask] = math.nan, math.inf
+    for t in (q2, k2, v2, d2):
+        t[:5], t[cu[-1]:] = math.nan, math.nan
+    d2[cu[1]:cu[2]] = math.inf  # queries without a key
+    for a, b in zip(got, attention_all(q2, k2, v2, cut, d2, mask=mask)):
+        assert torch.equal(a, b)
+
+
+def test_attention_scales_and_large_scores():
+    """Scores of several hundred (one key takes all), a tiny scale (all keys alike), values of 1e4."""
+    for gain, scale in ((60.0, None), (1.0, 1e-4), (1.0, 2.0)):
+        q, k, v, cu, cut, dout, _ = attention_inputs(9, [130, 70], 2, 2, 64, q_gain=gain)
+        check_attention(q, k, v, cu, cut, dout, scale)
+    q, k, v, cu, cut, dout, _ = attention_inputs(10, [130, 70], 2, 2, 64)
+    check_attention(q, k, (v * 1e4).bfloat16(), cu, cut, dout)
+
+
+def test_attention_layouts():
+    """Head-major storage, an unaligned slice (copied), int strides past 2^31 elements."""
+    q, k, v, cu, cut, dout, _ = attention_inputs(21, [90, 33], 4, 2, 64)
+    base = attention_all(q.contiguous(), k.contiguous(), v.contiguous(), cut, dout)
+    hm = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    odd = torch.empty(len(q), 4, 65, dtype=torch.bfloat16, device="cuda")[:, :, 1:]
+    odd.copy_(q)
+    one = dout[:, :1].expand(-1, 4, -1)
+    for args in ((q, k, v, dout), (hm(q), hm(k), hm(v), hm(dout)), (odd, k, v, dout)):
+        for a, b in zip(base, attention_all(*args[:3], cut, args[3])):
+            assert torch.equal(a, b)
+    for a, b in zip(attention_all(q, k, v, cut, one), attention_all(q, k, v, cut, one.contiguous())):
+        assert torch.equal(a, b)
+    N = 400
+    big = torch.empty(N * (2 ** 23 - 8), dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((N, 3, 64), (2 ** 23 - 8, 64, 1))
+    far.copy_(randn(gen(2), N, 3, 64))
+    cut = torch.tensor([0, 150, N], dtype=torch.int32, device="cuda")
+    near = far.contiguous()
+    d = dout.new_ones(N, 1, 64)
+    for a, b in zip(attention_all(far[:, :1], far[:, 1:2], far[:, 2:], cut, d), attention_all(near[:, :1], near[:, 1:2], near[:, 2:], cut, d)):
+        assert torch.equal(a, b)
+
+
+def test_attention_offsets_outside_the_buffer_are_clamped():
+    q, k, v, cu, cut, dout, _ = attention_inputs(4, [90, 60], 2, 2, 64)
+    bad = torch.tensor([-7, 90, 150 + 1000], dtype=torch.int32, device="cuda")
+    for a, b in zip(attention_all(q, k, v, cut, dout), attention_all(q, k, v, bad, dout)):
+        assert torch.equal(a, b)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = attention_all(q, k, v, none, dout)
+    assert (out[1] == -math.inf).all() and not any(t.any() for t in (out[0],) + out[2:])
+
+
+def test_attention_autograd_and_differences():
+    q, k, v, cu, cut, dout, g = attention_inputs(31, [70, 45], 4, 2, 64)
+    scale = 0.125
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    T().attention_varlen(*leaves, cut).backward(dout)
+    want, tol = attention_oracle(q, k, v, cu, scale, None, dout)
+    for i, (t, a, e) in enumerate(zip(leaves, want[2:], tol[2:])):
+        within(t.grad, a, e, "autograd")
+        d = randn(g, *t.shape).double()
+        f = lambda s: (attention_oracle(*[(x.double() + s * d if j == i else x) for j, x in enumerate((q, k, v))], cu, scale,
+                                        None, dout)[0][0] * dout.double()).sum().item()
+        slope = (f(1e-4) - f(-1e-4)) / 2e-4
+        assert abs((t.grad.double() * d).sum().item() - slope) <= (e * d.abs()).sum().item() + 1e-5 * (a.abs() * d.abs()).sum().item()
+
+
+# ------------------------------------------------------------------------------------------------ preference loss
+
+def preference_oracle(z, y, cu, ref, beta, eps, alpha, dtype):
+    """64-bit (loss, logps, dz) and bounds: a token's log-probability is off by u (V + 64 + 4 |logp| + 4 |z_y - max|) at most
+    (its sum has below V / 16 + 16 additions of terms that are off by 4 u (1 + |z - max|), and exp damps those)."""
+    z = z.double()
+    V = z.shape[1]
+    P = (len(cu) - 1) // 2
+    lp = torch.log_softmax(z, -1)
+    l, tl, n = [], [], []
+    used = []
+    for a, b in zip(cu, cu[1:]):
+        rows = torch.arange(a, b, device=z.device)
+        rows = rows[(y[rows] >= 0) & (y[rows] < V)]
+        x = lp[rows, y[rows]]
+        l.append(x.sum())
+        tl.append((U * (V / 16 + 64 + 8 * x.abs())).sum() + U * x.sum().abs())
+        n.append(max(1, len(rows)))
+        used.append(rows)
+    ref = ref.double()
+    loss, tloss, dz, tdz = 0.0, 0.0, torch.zeros_like(z), torch.zeros_like(z)
+    r = R[dtype]
+    for i in range(P):
+        m = beta * ((l[2 * i] - ref[2 * i]) - (l[2 * i + 1] - ref[2 * i + 1]))
+        tm = abs(beta) * (tl[2 * i] + tl[2 * i + 1])
+        sp = lambda t: torch.nn.functional.softplus(t, threshold=1e9)
+        loss = loss + ((1 - eps) * sp(-m) + eps * sp(m) - alpha * l[2 * i] / n[2 * i]) / P
+        tloss = tloss + (tm + abs(alpha) * tl[2 * i] / n[2 * i]) / P
+        gm = beta * (eps * torch.sigmoid(m) - (1 - eps) * torch.sigmoid(-m)) / P
+        tg = abs(beta) * tm / 4 / P
+        for j, c in ((2 * i, gm - alpha / n[2 * i] / P), (2 * i + 1, -gm)):
+            rows = used[j]
+            p = lp[rows].exp()
+            hot = torch.nn.functional.one_hot(y[rows], V).double()
+            dz[rows] = c * (hot - p)
+            ep = p * U * (V / 16 + 64 + 8 * lp[rows].abs())
+            tdz[rows] = (tg + 4 * U * abs(c)) * (hot - p).abs() + abs(c) * (ep + U * hot)
+    tdz = tdz * (1 + r) + r * dz.abs() + 2e-38  # results below the smallest normal number may be flushed
+    return (loss, torch.stack(l), dz), (tloss + 4 * U * abs(loss), torch.stack(tl) + U * torch.stack(l).abs(), tdz)
+
+
+def preference_inputs(seed, lens, V, dtype, tail=0, spread=1.5):
+    g = gen(seed)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    N = cu[-1] + tail
+    z = (spread * randn(g, N, V)).to(dtype)
+    y = torch.randint(0, V, (N,), generator=g, device="cuda")
+    y[torch.rand(N, generator=g, device="cuda") < 0.25] = -100
+    ref = -3.0 * torch.tensor([float(n) for n in lens], device="cuda") + randn(g, len(lens))
+    return z, y, cu, torch.tensor(cu, dtype=torch.int32, device="cuda"), ref, g
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,lens,tail", [(64, [5, 9], 0), (64, [1, 0, 0, 3], 2), (1, [4, 4], 0), (2, [3, 3], 0), (33, [70, 64, 1, 130], 7),
+                                         (256, [40, 40], 0), (257, [17, 33], 1), (4096, [30, 41], 0), (4101, [20, 9, 11, 1], 5),
+                                         (9001, [3, 2], 0), (64, [7] * 140, 0)])
+def test_preference_loss(V, lens, tail, dtype):
+    z, y, cu, cut, ref, _ = preference_inputs(V + len(lens), lens, V, dtype, tail)
+    if len(y) > 6:
+        y[3] = V  # out of range: not scored
+    for beta, eps, alpha in ((0.1, 0.0, 0.0), (0.5, 0.1, 0.3), (0.05, 1.0, 1.0)):
+        loss, logps, saved = T().preference_loss_forward(z, y, cut, ref, beta, eps, alpha)
+        dz = T().preference_loss_backward(z, y, saved)
+        want, tol = preference_oracle(z, y, cu, ref, beta, eps, alpha, dtype)
+        for got, a, t, n in zip((loss, logps, dz), want, tol, ("loss", "logps", "dz")):
+            within(got, a, t, n)
+        assert dz.dtype == dtype and not dz[(y < 0) | (y >= V)].any() and not dz[cu[-1]:].any()
+
+
+def test_preference_skipped_tokens_may_hold_anything():
+    z, y, cu, cut, ref, _ = preference_inputs(8, [20, 30, 10, 15], 65, torch.float32, tail=9)
+    a = T().preference_loss_forward(z, y, cut, ref, 0.1, 0.1, 0.5)
+    z2, y2 = z.clone(), y.clone()
+    z2[y < 0] = math.nan
+    z2[cu[-1]:] = math.inf
+    b = T().preference_loss_forward(z2, y2, cut, ref, 0.1, 0.1, 0.5)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(T().preference_loss_backward(z, y, a[2]), T().preference_loss_backward(z2, y2, b[2]))
+    # vocabulary entries that are ruled out (-inf, or the type's lowest value), and a long way between logits
+    for fill in (-math.inf, torch.finfo(torch.float32).min):
+        z3 = z.clone()
+        z3[:, ::3] = fill
+        y3 = torch.where(y % 3 == 0, torch.full_like(y, -100), y)
+        for s in (1.0, 200.0):
+            zs = torch.where(z3 == fill, z3, z3 * s)
+            got = T().preference_loss_forward(zs, y3, cut, ref)
+            dz = T().preference_loss_backward(zs, y3, got[2])
+            zo = zs.double().masked_fill(z3 == fill, -1e30)
+            want, tol = preference_oracle(zo, y3, cu, ref, 0.1, 0.0, 0.0, torch.float32)
+            keep = z3 != fill
+            within(got[0], want[0], tol[0], "loss")
+            assert not dz[~keep].any()
+            within(dz[keep], want[2][keep], tol[2][keep], "dz")
+
+
+def test_preference_autograd_and_differences():
+    z, y, cu, cut, ref, g = preference_inputs(13, [25, 31, 12, 40], 64, torch.float32)
+    x = z.clone().requires_grad_()
+    loss, logps = T().preference_loss(x, y, cut, ref, beta=0.3, label_smoothing=0.1, nll_weight=0.2)
+    assert loss.requires_grad and not logps.requires_grad
+    (loss * 2.5).backward()
+    want, tol = preference_oracle(z, y, cu, ref, 0.3, 0.1, 0.2, torch.float32)
+    within(x.grad, 2.5 * want[2], 2.5 * tol[2] + 2 * U * 2.5 * want[2].abs(), "autograd")
+    v = randn(g, *z.shape).double()
+    f = lambda s: preference_oracle(z.double() + s * v, y, cu, ref, 0.3, 0.1, 0.2, torch.float32)[0][0].item()
+    slope = 2.5 * (f(1e-4) - f(-1e-4)) / 2e-4
+    assert abs((x.grad.double() * v).sum().item() - slope) <= 3 * (tol[2] * v.abs()).sum().item() + 1e-6 * (want[2].abs() * v.abs()).sum().item()
+
+
+# ------------------------------------------------------------------------------------------------ together
+
+class Block:
+    """A pre-norm attention sublayer (reference esm/layers/attention.py:26-33, blocks.py:146-155) and a vocabulary head."""
+
+    def __init__(self, d, H, V, seed, dtype=torch.float32):
+        g = gen(seed)
+        p = lambda *s, m=0.0, w=0.1: (m + w * randn(g, *s)).to(dtype)
+        self.d, self.H = d, H
+        self.p = {"ln_w": p(d, m=1), "ln_b": p(d), "w_qkv": p(3 * d, d, w=d ** -0.5), "q_ln": p(d, m=1), "k_ln": p(d, m=1),
+                  "w_o": p(d, d, w=d ** -0.5), "f_ln": p(d, m=1), "w_v": p(V, d, w=d ** -0.5)}
+
+    def run(self, x, p, norm, attend):
+        N, d = x.shape
+        qkv = norm(x, p["ln_w"], p["ln_b"]) @ p["w_qkv"].t()
+        q, k, v = norm(qkv[:, :d], p["q_ln"], None), norm(qkv[:, d:2 * d], p["k_ln"], None), qkv[:, 2 * d:]
+        heads = lambda t: t.reshape(N, self.H, d // self.H)
+        x = x + attend(heads(q), heads(k), heads(v)).reshape(N, d) @ p["w_o"].t()
+        return norm(x, p["f_ln"], None) @ p["w_v"].t()
+
+
+def plain_norm(x, w, b):
+    h = (x - x.mean(-1, keepdim=True)) / ((x - x.mean(-1, keepdim=True)).pow(2).mean(-1, keepdim=True) + 1e-5).sqrt()
+    return h * w + (0 if b is None else b)
+
+
+def plain_attend(cu, keep):
+    def go(q, k, v):
+        out = torch.zeros_like(q)
+        for a, b in zip(cu, cu[1:]):
+            s = torch.einsum("qhd,khd->hqk", q[a:b], k[a:b]) * q.shape[2] ** -0.5
+            s = s.masked_fill(~keep[a:b], -math.inf)
+            out = torch.cat([out[:a], torch.einsum("hqk,khd->qhd", s.softmax(-1), v[a:b]), out[b:]])
+        return out
+    return go
+
+
+def test_preference_step_through_a_block():
+    """Loss and every parameter's gradient of norm -> qkv -> q/k norm -> attention -> residual -> norm -> head -> loss against
+    64-bit autograd.  The bf16 roundings on the way (eleven per path: activations, q k v, P, dS, their gradients) are
+    independent: relative errors of sqrt(11) 2^-8 = 1.3 % of the norm at most; 2 % is asked."""
+    d, H, V = 128, 2, 64
+    blk = Block(d, H, V, 1)
+    z, y, cu, cut, ref, g = preference_inputs(17, [60, 75, 130, 20], V, torch.float32)
+    N = cu[-1]
+    keep = torch.rand(N, generator=g, device="cuda") > 0.2
+    keep[cu[:-1]] = True
+    x0 = randn(g, N, d)
+    ref = -4.0 * torch.tensor([60.0, 75, 130, 20], device="cuda") * 0.75
+    p16 = {n: t.clone().requires_grad_() for n, t in blk.p.items()}
+    bf = lambda x, w, b: T().layer_norm(x.bfloat16(), w, b)
+    low = {n: (t if "ln" in n else t.bfloat16()) for n, t in p16.items()}
+    logits = blk.run(x0.bfloat16(), low, bf, lambda q, k, v: T().attention_varlen(q, k, v, cut, key_mask=keep))
+    loss, logps = T().preference_loss(logits.float(), y, cut, ref, nll_weight=0.1)
+    loss.backward()
+    p64 = {n: (t.double() if "ln" in n else t.bfloat16().double()).requires_grad_() for n, t in blk.p.items()}
+    lg = blk.run(x0.bfloat16().double(), p64, plain_norm, plain_attend(cu, keep))
+    lp = torch.log_softmax(lg, -1)
+    l = torch.stack([lp[a:b][y[a:b] >= 0].gather(1, y[a:b][y[a:b] >= 0][:, None]).sum() for a, b in zip(cu, cu[1:])])
+    m = 0.1 * ((l - ref)[0::2] - (l - ref)[1::2])
+    n = torch.tensor([int((y[a:b] >= 0).sum()) for a, b in zip(cu, cu[1:])], device="cuda")
+    want = (torch.nn.functional.softplus(-m) - 0.1 * l[0::2] / n[0::2]).mean()
+    want.backward()
+    assert abs(loss.item() - want.item()) <= 0.02 * abs(want.item())
+    assert (logps.double() - l).norm() <= 0.02 * l.norm()
+    for name, t in p16.items():
+        g64 = p64[name].grad
+        assert (t.grad.double() - g64).norm() <= 0.02 * g64.norm(), name
+
+
+def _step(x, dy, w, b, q, k, v, cu, dout, mask, z, y, cp, ref):
+    n, st = T().layer_norm_forward(x, w, b)
+    got = [n, st, *T().layer_norm_backward(dy, x, w, st)]
+    got += attention_all(q, k, v, cu, dout, mask=mask)
+    loss, lp, saved = T().preference_loss_forward(z, y, cp, ref, nll_weight=0.5)
+    return got + [loss, lp, T().preference_loss_backward(z, y, saved)]
+
+
+def _step_inputs(seed):
+    g = gen(seed)
+    q, k, v, _, cu, dout, _ = attention_inputs(seed, [100, 31, 200], 4, 2, 64, tail=3)
+    z, y, _, cp, ref, _ = preference_inputs(seed, [40, 50, 33, 21], 64, torch.float32)
+    return [randn(g, 600, 384).bfloat16(), randn(g, 600, 384).bfloat16(), 1 + 0.1 * randn(g, 384), randn(g, 384), q, k, v, cu,
+            dout, torch.rand(len(q), generator=g, device="cuda") > 0.1, z, y, cp, ref]
+
+
+def test_same_bits_again_on_other_streams_and_in_a_replayed_graph():
+    a, b = _step_inputs(1), _step_inputs(2)
+    b[7], b[12] = a[7], a[12]
+    ea, eb = _step(*a), _step(*b)
+    for p, q in zip(ea, _step(*a)):
+        assert torch.equal(p, q)
+    # two streams at once, each with its own outputs and scratch memory
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for s, args in ((s1, a), (s2, b), (s1, b), (s2, a)):
+        with torch.cuda.stream(s):
+            got.append(_step(*args))
+    torch.cuda.synchronize()
+    for out, want in zip(got, (ea, eb, eb, ea)):
+        for p, q in zip(out, want):
+            assert torch.equal(p, q)
+    # one captured step, replayed with other inputs in its buffers and eager work in between
+    bufs = [t.clone() for t in a]
+    with torch.cuda.stream(s1):
+        _step(*bufs)
+    torch.cuda.synchronize()
+    graph, graph2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = _step(*bufs)
+    with torch.cuda.graph(graph2):
+        outs2 = _step(*b)
+    for args, want in ((b, eb), (a, ea), (b, eb)):
+        for t, s in zip(bufs, args):
+            t.copy_(s)
+        graph.replay()
+        graph2.replay()
+        mid = _step(*a)
+        torch.cuda.synchronize()
+        for o, w in ((outs, want), (outs2, eb), (mid, ea)):
+            for p, q in zip(o, w):
+                assert torch.equal(p, q)
+
+
+def test_refusals_name_the_argument():
+    t = T()
+    x, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    q = torch.zeros(8, 2, 64, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    y = torch.zeros(8, dtype=torch.int64, device="cuda")
+    z = torch.zeros(8, 16, device="cuda")
+    cp, ref = torch.tensor([0, 4, 8], dtype=torch.int32, device="cuda"), torch.zeros(2, device="cuda")
+    y0, st = t.layer_norm_forward(x, w)
+    o, lse = t.attention_varlen_forward(q, q, q, cu)
+    for err, call in (
+            (ValueError, lambda: t.layer_norm_forward(x, w[:32])), (ValueError, lambda: t.layer_norm_forward(x, w, w[:1])),
+            (TypeError, lambda: t.layer_norm_forward(x.half(), w)), (ValueError, lambda: t.layer_norm_backward(x[:2], x, w, st)),
+            (TypeError, lambda: t.layer_norm_backward(x.bfloat16(), x, w, st)),
+            (ValueError, lambda: t.layer_norm_backward(x, x, w, st[:2])),
+            (ValueError, lambda: t.layer_norm_forward(torch.zeros(1, 12289, device="cuda"), torch.ones(12289, device="cuda"))),
+            (TypeError, lambda: t.attention_varlen_forward(q.float(), q, q, cu)),
+            (ValueError, lambda: t.attention_varlen_forward(q[:, :, :32], q[:, :, :32], q[:, :, :32], cu)),
+            (ValueError, lambda: t.attention_varlen_forward(q, q[:, :1].expand(8, 3, 64), q[:, :1].expand(8, 3, 64), cu)),
+            (ValueError, lambda: t.attention_varlen_forward(q, q[:4], q[:4], cu)),
+            (TypeError, lambda: t.attention_varlen_forward(q, q, q, cu.long())),
+            (ValueError, lambda: t.attention_varlen_forward(q, q, q, cu, scale=-1.0)),
+            (ValueError, lambda: t.attention_varlen_forward(q, q, q, cu, scale=0.0)),
+            (ValueError, lambda: t.attention_varlen_forward(q, q, q, cu, key_mask=torch.ones(7, dtype=torch.bool, device="cuda"))),
+            (ValueError, lambda: t.attention_varlen_backward(o, q, q, q, o, lse[:1], cu)),
+            (ValueError, lambda: t.preference_loss_forward(z, y[:4], cp, ref)),
+            (ValueError, lambda: t.preference_loss_forward(z, y, cu, ref)),
+            (ValueError, lambda: t.preference_loss_forward(z, y, cp, ref[:1])),
+            (ValueError, lambda: t.preference_loss_forward(z, y, cp, ref, label_smoothing=1.5)),
+            (TypeError, lambda: t.preference_loss_forward(z, y.int(), cp, ref)),
+            (ValueError, lambda: t.preference_loss_backward(z, y, torch.zeros(8, dtype=torch.uint8, device="cuda")))):
+        with pytest.raises(err):
+            call()
