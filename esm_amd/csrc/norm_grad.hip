@@ -4,7 +4,8 @@
 //   h = (x - mean) rstd,  y = h gamma + beta
 //   g = dy gamma,  dx = rstd (g - mean_d(g) - h mean_d(g h)),  dgamma = sum_rows dy h,  dbeta = sum_rows dy
 //
-// Both are bound by HBM: the forward pass has to move 2 M d elements, the backward pass 3 M d.  WPR waves share a row
+// Both are bound by HBM: the forward pass has to move 2 M d elements, the backward pass 3 M d.  At 32768 x 1152 bf16 the
+// forward pass takes 30 us (5.0 TB/s; a copy of the same size 5.0), the backward pass 42 + 5 us (5.4 TB/s).  WPR waves share a row
 // and keep all of it in registers (one read), sums run in fp32, and the next row's loads are in flight while the current
 // one is reduced.  A lane owns the same columns of every row it meets, so it sums its columns of dgamma / dbeta in
 // registers; each workgroup leaves one partial row, and a second kernel adds the partial rows in a fixed order (no
@@ -16,21 +17,30 @@
 namespace {
 
 constexpr int NG_MAX_D = 12288;      // 8 waves x 64 lanes x 24 elements
-constexpr int NG_MAX_GROUPS = 512;   // partial rows of dgamma / dbeta
+constexpr int NG_FWD_GROUPS = 1024;  // four workgroups per CU; 512 to 2048 measure alike
+constexpr int NG_MAX_GROUPS = 512;   // of the backward pass, and so partial rows; 768 and 1024: 2 to 10 % slower
 
 template <typename T> struct NgVec;  // 16 bytes of T
 template <> struct NgVec<float> { static constexpr int N = 4; };
 template <> struct NgVec<__bf16> { static constexpr int N = 8; };
 
-// VEC elements of a row: one 16-byte load, or one element where width, stride or address rule that out
+// VEC elements of a row: 16 bytes, or one element where width, stride or address rule that out.  Rows go through buffer
+// descriptors that end where the row ends: a lane past the end reads zeros and its stores are dropped, so neither loop has
+// a branch around its loads and stores (with branches the compiler cannot count what is in flight and waits for all of it:
+// the forward pass took 54 us at 32768 x 1152 bf16 that way).
 template <typename T, int VEC> struct NgRaw { u32x4 v; };
-template <> struct NgRaw<float, 1> { float v; };
+template <> struct NgRaw<float, 1> { unsigned v; };
 template <> struct NgRaw<__bf16, 1> { unsigned short v; };
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t ng_row(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
+}
 template <typename T, int VEC>
-__device__ __forceinline__ NgRaw<T, VEC> ng_load(const T* p) {
+__device__ __forceinline__ NgRaw<T, VEC> ng_load(__amdgpu_buffer_rsrc_t row, int off) {
     NgRaw<T, VEC> r;
-    r.v = *(const decltype(r.v)*)p;
+    if constexpr (VEC > 1) r.v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(row, off, 0, 0));
+    else if constexpr (sizeof(T) == 4) r.v = __builtin_amdgcn_raw_buffer_load_b32(row, off, 0, 0);
+    else r.v = __builtin_amdgcn_raw_buffer_load_b16(row, off, 0, 0);
     return r;
 }
 __device__ __forceinline__ void ng_unpack(const NgRaw<float, 4>& r, float* f) {
@@ -44,25 +54,57 @@ __device__ __forceinline__ void ng_unpack(const NgRaw<__bf16, 8>& r, float* f) {
         f[2 * e + 1] = __uint_as_float(r.v[e] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void ng_unpack(const NgRaw<float, 1>& r, float* f) { f[0] = r.v; }
+__device__ __forceinline__ void ng_unpack(const NgRaw<float, 1>& r, float* f) { f[0] = __uint_as_float(r.v); }
 __device__ __forceinline__ void ng_unpack(const NgRaw<__bf16, 1>& r, float* f) { f[0] = bf16_bits_to_f32(r.v); }
-__device__ __forceinline__ void ng_store(float* p, const float (&f)[4]) { *(f32x4*)p = f32x4{f[0], f[1], f[2], f[3]}; }
-__device__ __forceinline__ void ng_store(__bf16* p, const float (&f)[8]) {
-    *(u32x4*)p = u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
+template <typename T, int VEC>
+__device__ __forceinline__ void ng_store(__amdgpu_buffer_rsrc_t row, int off, const float (&f)[VEC]) {
+    if constexpr (VEC == 8)
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])}, row, off, 0, 0);
+    else if constexpr (VEC == 4)
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}, row, off, 0, 0);
+    else if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(f[0]), row, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16_bits(f[0]), row, off, 0, 0);
 }
-__device__ __forceinline__ void ng_store(float* p, const float (&f)[1]) { *p = f[0]; }
-__device__ __forceinline__ void ng_store(__bf16* p, const float (&f)[1]) { *p = (__bf16)f[0]; }
+// VEC fp32 parameters
+template <int VEC>
+__device__ __forceinline__ void ng_param(const float* p, int d, int off, float (&f)[VEC]) {
+    const __amdgpu_buffer_rsrc_t r = ng_row(p, p ? d * 4 : 0);
+#pragma unroll
+    for (int e = 0; e < VEC; e += VEC > 1 ? 4 : 1) {
+        if constexpr (VEC > 1) {
+            const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (off + e) * 4, 0, 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[e + i] = __uint_as_float(v[i]);
+        } else {
+            f[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (off + e) * 4, 0, 0));
+        }
+    }
+}
 
 // Threads of a workgroup: four waves, eight where eight waves share a row.
 constexpr int ng_threads(int wpr) { return wpr == 8 ? 512 : 256; }
+
+// Sum over the 64 lanes, the same in all of them, on the vector ALU alone (DPP within 16 lanes, then the half-row and
+// half-wave swaps): a row waits for two such sums, and through the LDS crossbar each of their six steps costs its latency.
+__device__ __forceinline__ float lane_sum(float v) {
+    auto step = [&](auto ctrl) { v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false)); };
+    step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+    step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+    step(std::integral_constant<int, 0x141>{});  // mirrored in 8
+    step(std::integral_constant<int, 0x140>{});  // mirrored in 16
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
 
 // Sum of (a, b) over the WPR waves of a row.  `buf` holds one pair per wave and alternates between two halves, so that
 // one barrier per call is enough: a wave reaches the call after next only behind the barrier that every reader of the
 // earlier half has passed.  All waves of the workgroup call it equally often.
 template <int WPR>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float* buf, int& half) {
-    a = wave_sum(a);
-    b = wave_sum(b);
+    a = lane_sum(a);
+    b = lane_sum(b);
     if constexpr (WPR > 1) {
         const int wave = threadIdx.x >> 6;
         float* p = buf + half * 16;
@@ -82,59 +124,61 @@ __global__ __launch_bounds__(ng_threads(WPR)) void norm_fwd_kernel(const T* __re
                                                                    const float* __restrict__ beta, T* __restrict__ y,
                                                                    float* __restrict__ stats, int M, int d, float eps) {
     constexpr int ROWS = ng_threads(WPR) / 64 / WPR;  // rows a workgroup works on at once
+    constexpr int STEP = 64 * WPR * VEC;              // elements between a lane's vectors
     __shared__ float buf[32];
-    const int lane = threadIdx.x & (64 * WPR - 1), slot = threadIdx.x / (64 * WPR);
-    const int nvec = d / VEC;
-    const int stride = gridDim.x * ROWS;
+    const int lane = threadIdx.x & (64 * WPR - 1);
+    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));
+    const int stride = gridDim.x * ROWS, bytes = d * (int)sizeof(T);
+    const float inv_d = 1.0f / (float)d;
     int half = 0;
     NgRaw<T, VEC> raw[NV];
     auto load = [&](int r) {
+        const __amdgpu_buffer_rsrc_t xr = ng_row(x + (r < M ? r : 0) * ldx, r < M ? bytes : 0);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + i * 64 * WPR < nvec) raw[i] = ng_load<T, VEC>(x + (int64_t)r * ldx + lane * VEC + i * 64 * WPR * VEC);
+        for (int i = 0; i < NV; ++i) raw[i] = ng_load<T, VEC>(xr, (lane * VEC + i * STEP) * (int)sizeof(T));
     };
-    int first = blockIdx.x * ROWS;  // uniform over the workgroup: every wave makes the same number of turns
-    if (first + slot < M) load(first + slot);
-    for (; first < M; first += stride) {
-        const int row = first + slot;
-        const bool on = row < M;
+    int row = blockIdx.x * ROWS + slot;
+    load(row);
+    __builtin_amdgcn_sched_barrier(0);  // the row first: the loop then waits for loads by count, not for stores
+    float w[NV][VEC], b[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        ng_param<VEC>(gamma, d, lane * VEC + i * STEP, w[i]);
+        ng_param<VEC>(beta, d, lane * VEC + i * STEP, b[i]);
+    }
+    for (; row - slot < M; row += stride) {  // the same number of turns in every wave of the workgroup
         float v[NV][VEC], sum = 0.f, none = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (on && lane + i * 64 * WPR < nvec) ng_unpack(raw[i], v[i]);
-            else
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[i][e] = 0.f;
+            ng_unpack(raw[i], v[i]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) sum += v[i][e];
         }
-        if (row + stride < M) load(row + stride);
+        load(row + stride < M ? row + stride : M);
         row_sum2<WPR>(sum, none, buf, half);
-        const float mean = sum / (float)d;
+        const float mean = sum * inv_d;
         float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + i * 64 * WPR < nvec)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    v[i][e] -= mean;
-                    sq += v[i][e] * v[i][e];
-                }
-        row_sum2<WPR>(sq, none, buf, half);
-        const float rstd = 1.0f / sqrtf(sq / (float)d + eps);
-        if (!on) continue;
-        if (lane == 0) *(f32x2*)(stats + 2 * (int64_t)row) = f32x2{mean, rstd};
-#pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = lane + i * 64 * WPR;
-            if (c >= nvec) continue;
-            float o[VEC];
+            const bool in = lane * VEC + i * STEP < d;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float b = beta ? beta[c * VEC + e] : 0.f;
-                o[e] = v[i][e] * rstd * gamma[c * VEC + e] + b;
+                v[i][e] = in ? v[i][e] - mean : 0.f;
+                sq += v[i][e] * v[i][e];
             }
-            ng_store(y + (int64_t)row * d + lane * VEC + i * 64 * WPR * VEC, o);
+        }
+        row_sum2<WPR>(sq, none, buf, half);
+        const float rstd = 1.0f / sqrtf(sq * inv_d + eps);
+        const int at = row < M ? row : 0;
+        const __amdgpu_buffer_rsrc_t sr = ng_row(stats + 2 * (int64_t)at, row < M ? 8 : 0);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(mean), __float_as_uint(rstd)}, sr, lane * 8, 0, 0);
+        const __amdgpu_buffer_rsrc_t yr = ng_row(y + (int64_t)at * d, row < M ? bytes : 0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = v[i][e] * rstd * w[i][e] + b[i][e];
+            ng_store<T, VEC>(yr, (lane * VEC + i * STEP) * (int)sizeof(T), o);
         }
     }
 }
@@ -146,58 +190,49 @@ __global__ __launch_bounds__(ng_threads(WPR)) void norm_bwd_kernel(const T* __re
                                                                    const float* __restrict__ stats, T* __restrict__ dx,
                                                                    float* __restrict__ pg, float* __restrict__ pb, int M,
                                                                    int d) {
-    constexpr int ROWS = ng_threads(WPR) / 64 / WPR;
+    constexpr int ROWS = ng_threads(WPR) / 64 / WPR, STEP = 64 * WPR * VEC;
     __shared__ float buf[32];
     extern __shared__ float part[];  // [ROWS - 1][2][d]
-    const int lane = threadIdx.x & (64 * WPR - 1), slot = threadIdx.x / (64 * WPR);
-    const int nvec = d / VEC;
-    const int stride = gridDim.x * ROWS;
+    const int lane = threadIdx.x & (64 * WPR - 1);
+    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));
+    const int stride = gridDim.x * ROWS, bytes = d * (int)sizeof(T);
     const float inv_d = 1.0f / (float)d;
     int half = 0;
     NgRaw<T, VEC> rx[NV], rg[NV];
     float mean = 0.f, rstd = 0.f;
     auto load = [&](int r) {
-        const f32x2 st = *(const f32x2*)(stats + 2 * (int64_t)r);
-        mean = st[0];
-        rstd = st[1];
+        const int at = r < M ? r : 0;
+        const int n = r < M ? bytes : 0;
+        const __amdgpu_buffer_rsrc_t xr = ng_row(x + at * ldx, n), gr = ng_row(dy + at * lddy, n);
+        mean = r < M ? stats[2 * (int64_t)at] : 0.f;
+        rstd = r < M ? stats[2 * (int64_t)at + 1] : 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (lane + i * 64 * WPR < nvec) {
-                rx[i] = ng_load<T, VEC>(x + (int64_t)r * ldx + lane * VEC + i * 64 * WPR * VEC);
-                rg[i] = ng_load<T, VEC>(dy + (int64_t)r * lddy + lane * VEC + i * 64 * WPR * VEC);
-            }
+            rx[i] = ng_load<T, VEC>(xr, (lane * VEC + i * STEP) * (int)sizeof(T));
+            rg[i] = ng_load<T, VEC>(gr, (lane * VEC + i * STEP) * (int)sizeof(T));
         }
     };
+    int row = blockIdx.x * ROWS + slot;
+    load(row);
+    __builtin_amdgcn_sched_barrier(0);
     float w[NV][VEC], ag[NV][VEC], ab[NV][VEC];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = lane + i * 64 * WPR;
+        ng_param<VEC>(gamma, d, lane * VEC + i * STEP, w[i]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            ag[i][e] = ab[i][e] = 0.f;
-            w[i][e] = c < nvec ? gamma[c * VEC + e] : 0.f;
-        }
+        for (int e = 0; e < VEC; ++e) ag[i][e] = ab[i][e] = 0.f;
     }
-    int first = blockIdx.x * ROWS;
-    if (first + slot < M) load(first + slot);
-    for (; first < M; first += stride) {
-        const int row = first + slot;
-        const bool on = row < M;
+    for (; row - slot < M; row += stride) {
         float h[NV][VEC], g[NV][VEC], c1 = 0.f, c2 = 0.f;
         const float rs = rstd;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (on && lane + i * 64 * WPR < nvec) {
-                ng_unpack(rx[i], h[i]);
-                ng_unpack(rg[i], g[i]);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) h[i][e] = (h[i][e] - mean) * rs;
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) h[i][e] = g[i][e] = 0.f;
-            }
+            // past the row's end, and in a row past the last, dy reads as zero: nothing is added anywhere (h is finite there)
+            ng_unpack(rx[i], h[i]);
+            ng_unpack(rg[i], g[i]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
+                h[i][e] = (h[i][e] - mean) * rs;
                 ag[i][e] += g[i][e] * h[i][e];
                 ab[i][e] += g[i][e];
                 g[i][e] *= w[i][e];
@@ -205,54 +240,67 @@ __global__ __launch_bounds__(ng_threads(WPR)) void norm_bwd_kernel(const T* __re
                 c2 += g[i][e] * h[i][e];
             }
         }
-        if (row + stride < M) load(row + stride);
+        load(row + stride < M ? row + stride : M);
         row_sum2<WPR>(c1, c2, buf, half);
-        if (!on) continue;
         c1 *= inv_d;
         c2 *= inv_d;
+        const __amdgpu_buffer_rsrc_t dr = ng_row(dx + (int64_t)(row < M ? row : 0) * d, row < M ? bytes : 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = lane + i * 64 * WPR;
-            if (c >= nvec) continue;
             float o[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) o[e] = (g[i][e] - c1 - h[i][e] * c2) * rs;
-            ng_store(dx + (int64_t)row * d + lane * VEC + i * 64 * WPR * VEC, o);
+            ng_store<T, VEC>(dr, (lane * VEC + i * STEP) * (int)sizeof(T), o);
         }
     }
     if (!pg && !pb) return;
     // the workgroup's row slots, added in order
+    constexpr int Q = VEC > 1 ? 4 : 1;  // floats per LDS access
+    typedef float fq __attribute__((ext_vector_type(Q)));
     if (slot > 0) {
-        float* p = part + (int64_t)(slot - 1) * 2 * d;
+        float* p = part + (slot - 1) * 2 * d;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = lane + i * 64 * WPR;
-            if (c < nvec)
+            const int c = lane * VEC + i * STEP;
+            if (c < d)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) { p[c * VEC + e] = ag[i][e]; p[d + c * VEC + e] = ab[i][e]; }
+                for (int e = 0; e < VEC; e += Q) {
+                    fq u, v;
+#pragma unroll
+                    for (int j = 0; j < Q; ++j) { u[j] = ag[i][e + j]; v[j] = ab[i][e + j]; }
+                    *(fq*)(p + c + e) = u;
+                    *(fq*)(p + d + c + e) = v;
+                }
         }
     }
     __syncthreads();
-    if (slot == 0) {
+    if (slot > 0) return;
+    const __amdgpu_buffer_rsrc_t gr = ng_row(pg + (int64_t)blockIdx.x * d, pg ? d * 4 : 0);
+    const __amdgpu_buffer_rsrc_t br = ng_row(pb + (int64_t)blockIdx.x * d, pb ? d * 4 : 0);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = lane + i * 64 * WPR;
-            if (c < nvec)
+    for (int i = 0; i < NV; ++i) {
+        const int c = lane * VEC + i * STEP;
+        if (c < d)
+            for (int s = 0; s < ROWS - 1; ++s)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float a = ag[i][e], b = ab[i][e];
-                    for (int s = 0; s < ROWS - 1; ++s) {
-                        a += part[(int64_t)s * 2 * d + c * VEC + e];
-                        b += part[(int64_t)s * 2 * d + d + c * VEC + e];
-                    }
-                    if (pg) pg[(int64_t)blockIdx.x * d + c * VEC + e] = a;
-                    if (pb) pb[(int64_t)blockIdx.x * d + c * VEC + e] = b;
+                for (int e = 0; e < VEC; e += Q) {
+                    const fq u = *(const fq*)(part + s * 2 * d + c + e), v = *(const fq*)(part + s * 2 * d + d + c + e);
+#pragma unroll
+                    for (int j = 0; j < Q; ++j) { ag[i][e + j] += u[j]; ab[i][e + j] += v[j]; }
                 }
+#pragma unroll
+        for (int e = 0; e < VEC; e += Q) {
+            float u[Q], v[Q];
+#pragma unroll
+            for (int j = 0; j < Q; ++j) { u[j] = ag[i][e + j]; v[j] = ab[i][e + j]; }
+            ng_store<float, Q>(gr, (c + e) * 4, u);
+            ng_store<float, Q>(br, (c + e) * 4, v);
         }
     }
 }
 
-// Column sums of the G partial rows: 32 columns x 32 groups of rows per workgroup, then the groups in order.
+// Column sums of the G partial rows: 32 columns x 32 groups of rows per workgroup, then the groups in order.  A few
+// microseconds of latency: a group's rows are requested eight at a time.
 __global__ __launch_bounds__(1024) void norm_grad_reduce_kernel(const float* __restrict__ pg, const float* __restrict__ pb,
                                                                 float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                                 int G, int d) {
@@ -264,6 +312,7 @@ __global__ __launch_bounds__(1024) void norm_grad_reduce_kernel(const float* __r
     const int c = blockIdx.x * 32 + col;
     float a = 0.f;
     if (c < d)
+#pragma unroll 8
         for (int r = grp; r < G; r += 32) a += src[(int64_t)r * d + c];
     part[grp][col] = a;
     __syncthreads();
@@ -321,8 +370,8 @@ int norm_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, T* 
              hipStream_t s) {
     auto go = [&](auto vec, auto nv, auto wpr) {
         constexpr int V = decltype(vec)::value, N = decltype(nv)::value, W = decltype(wpr)::value;
-        const int rows = ng_rows(W), want = (M + rows - 1) / rows;
-        hipLaunchKernelGGL((norm_fwd_kernel<T, V, N, W>), dim3(want < 2048 ? want : 2048), dim3(ng_threads(W)), 0, s, x, ldx,
+        const int rows = ng_rows(W), want = (M + rows - 1) / rows, cap = NG_FWD_GROUPS;
+        hipLaunchKernelGGL((norm_fwd_kernel<T, V, N, W>), dim3(want < cap ? want : cap), dim3(ng_threads(W)), 0, s, x, ldx,
                            gamma, beta, y, stats, M, d, eps);
         return true;
     };
