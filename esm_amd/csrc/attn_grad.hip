@@ -52,9 +52,9 @@ __device__ __forceinline__ int swz(int r) {
 
 // LDS-DMA of one tile: a wave moves pieces of 1 KiB (64 lanes x 16 bytes, LDS side linear, swizzle on the source address).
 // Rows past `rows` are out of the descriptor's range and land as zeros.
-template <int D>
+template <int D, int ROWS = TR>
 struct Stage {
-    static constexpr int RB = 2 * D, CPR = D / 8, PIECES = TR * RB / 1024 / AG_WAVES;
+    static constexpr int RB = 2 * D, CPR = D / 8, PIECES = ROWS * RB / 1024 / AG_WAVES;
     unsigned off[PIECES];
     unsigned ldb;
     __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
@@ -67,7 +67,7 @@ struct Stage {
     }
     // first: first row of the tile (wave-uniform), rows: rows of it that exist (>= 1)
     __device__ __forceinline__ void go(char* lds, const __bf16* first, int rows, int wave) const {
-        const int nrec = (int)((rows < TR ? rows - 1 : TR - 1) * ldb + RB);
+        const int nrec = (int)((rows < ROWS ? rows - 1 : ROWS - 1) * ldb + RB);
         const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, nrec, 0x00020000);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
@@ -197,38 +197,77 @@ __device__ __forceinline__ void store_row(__bf16* row, const f32x16 (&o)[D / 32]
 
 // ---- which rows a block owns -------------------------------------------------------------------------------------------
 // The stretches of tokens are the sequences plus what lies before the first and behind the last.  Stretch e (0 .. n + 1)
-// starts at B(e) and gets block numbers from B(e) / BLK + e on: at least ceil(length / BLK) of them, so the grid
-// N / BLK + n + 2 is known without reading cu_seqlens, and a block finds its stretch by a 64-way search.  Offsets are
-// clamped into [0, N]: a bad cu_seqlens cannot lead outside the buffers.
+// starts at B(e) and gets block numbers from B(e) / 128 + e on: at least ceil(length / 128) of them, so the grid
+// N / 128 + n + 2 is known without reading cu_seqlens, and a block finds its stretch by search.  Offsets are clamped into
+// [0, N]: a bad cu_seqlens cannot lead outside the buffers.
+//
+// Order of the blocks: the blocks of a head over about one sequence are a group, and groups (all heads of a sequence, then
+// the next) are dealt to the eight XCDs in turn.  A group shares its keys in one XCD's L2, the XCDs together read whole rows
+// of a fused qkv buffer, and sequences of unequal length load all XCDs alike.  Within an XCD four groups advance together:
+// its workgroups go to its shader engines in turn, and a group's block numbers without rows would otherwise fall to the same
+// engines every time (128-token sequences: every second number; forward pass 118 -> 72 us).
+constexpr int AG_BLK = 128;  // rows a workgroup owns
+struct Order {
+    int n_blk, chunk, heads, grid;       // chunk: block numbers of an average sequence
+    unsigned by_chunk, by_heads;         // reciprocals, see quotient()
+    float per_blk;                       // stretches per block number
+};
 struct Span {
     int64_t s0;
     int len, first;  // rows of the stretch, first row of the block
     bool dead;       // no sequence: outputs are zeros
 };
-__device__ __forceinline__ Span find_span(int b, const int* __restrict__ cu, int n, int N, int blk) {
-    const int lane = threadIdx.x & 63;
-    auto start = [&](int e) { return e <= 0 ? 0 : e >= n + 2 ? N : min(max(cu[e - 1], 0), N); };
-    int lo = 0, cnt = n + 2;
-    while (cnt > 1) {
-        const int step = (cnt + 63) >> 6;
-        const int k = lane * step;
-        const unsigned long long m = __ballot(k < cnt && start(lo + k) / blk + lo + k <= b);
-        const int w = m ? 63 - __builtin_clzll(m) : 0;
-        lo += w * step;
-        cnt = min(step, cnt - w * step);
+// n / d with m = floor((2^32 - 1) / d): the product is at most one short
+__device__ __forceinline__ int quotient(int n, int d, unsigned m) {
+    const int q = (int)__umulhi((unsigned)n, m);
+    return n - q * d >= d ? q + 1 : q;
+}
+// false: no such block (uniform over the workgroup).  Everything here is on the scalar side, and for sequences of about
+// equal length one read of eight offsets settles it (a vector search took 4500 cycles of a 512-token block's 40000).
+__device__ __forceinline__ bool find_span(const Order& od, const int* __restrict__ cu, int n, int N, int& head, Span& s) {
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;  // blocks go to the XCDs round-robin
+    const int four = at >> 2, turn = quotient(four, od.chunk, od.by_chunk), group = (turn * 4 + (at & 3)) * 8 + xcd;
+    const int c = quotient(group, od.heads, od.by_heads);
+    head = group - c * od.heads;
+    const int b = c * od.chunk + (four - turn * od.chunk);
+    if (b >= od.n_blk) return false;
+    auto clamp = [&](int v) { return min(max(v, 0), N); };
+    auto start = [&](int e) { return e <= 0 ? 0 : e >= n + 2 ? N : clamp(cu[e - 1]); };
+    int lo = -1, a = 0, z = 0;
+    if (n >= 7) {  // cu has eight entries: those around where equal lengths would put the block
+        int g = (int)((float)b * od.per_blk) - 4;
+        g = min(max(g, 0), n - 7);
+        int v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = clamp(cu[g + i]);  // B(g + 1 + i)
+#pragma unroll
+        for (int i = 0; i < 7; ++i) {
+            const bool in = v[i] / AG_BLK + g + 1 + i <= b && b < v[i + 1] / AG_BLK + g + 2 + i;
+            lo = in ? g + 1 + i : lo;
+            a = in ? v[i] : a;
+            z = in ? v[i + 1] : z;
+        }
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    Span s;
-    const int a = start(lo), z = max(start(lo + 1), a);
+    if (lo < 0) {  // elsewhere: halving
+        lo = 0;
+        int hi = n + 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (start(mid) / AG_BLK + mid <= b) lo = mid;
+            else hi = mid - 1;
+        }
+        a = start(lo);
+        z = start(lo + 1);
+    }
     s.s0 = a;
-    s.len = z - a;
-    const int64_t first = (int64_t)(b - a / blk - lo) * blk;
-    s.first = first < s.len ? (int)first : s.len;
+    s.len = max(z - a, 0);
+    const int64_t first = (int64_t)(b - a / AG_BLK - lo) * AG_BLK;
     s.dead = lo == 0 || lo == n + 1;
-    return s;
+    s.first = (int)first;
+    return first < s.len;
 }
 
-// Keys of tile kt that take part, one bit each.
+// Which keys of a 64-key tile take part, one bit each; `row` is this lane's key.
 __device__ __forceinline__ unsigned char mask_byte(const unsigned char* mask, int64_t s0, int row, int len) {
     return row < len ? (mask ? mask[s0 + row] : 1) : 0;
 }
@@ -240,21 +279,92 @@ __device__ __forceinline__ void zero_rows(char* tile, unsigned long long bits) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) *(u32x4*)(tile + r * 2 * D + part * (D / 2) + i * 16) = u32x4{0u, 0u, 0u, 0u};
 }
+// Accumulator start of 32 scores from a row of 64 floats in LDS (0, or -inf where the key takes no part): masking costs
+// the row reads and no vector instruction.
+__device__ __forceinline__ f32x16 rows16(const float* st, int mt, int hi) {
+    f32x16 r;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 a = *(const f32x4*)(st + 32 * mt + 8 * g + 4 * hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[4 * g + e] = a[e];
+    }
+    return r;
+}
+__device__ __forceinline__ bf16x8 pack8(const float* f) {
+    return __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])});
+}
+
+// The key side of the forward and dQ kernels: K and V tiles through the ring, key masks, and the loop over the tiles.
+// MASK instantiations take every tile through the biased path; the others only a last tile that is not full, behind the
+// loop (one path inside the loop: a second one costs a copy of the accumulators per tile).
+template <int D, bool MASK, typename F>
+__device__ __forceinline__ void for_key_tiles(const View& k, const View& v, const unsigned char* mask, const Span& sp, int kvh,
+                                              char* smem, float (*bias)[TR], int wave, int lane, F tile) {
+    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
+    const __bf16* kb = k.p + sp.s0 * k.tok + kvh * k.head;
+    const __bf16* vb = v.p + sp.s0 * v.tok + kvh * v.head;
+    Stage<D> sk, sv;
+    sk.init(k.tok, wave, lane);
+    sv.init(v.tok, wave, lane);
+    const int nt = (sp.len + TR - 1) / TR;
+    auto stage = [&](int slot, int kt) {
+        char* base = smem + slot;
+        sk.go(base, kb + (int64_t)kt * TR * k.tok, sp.len - kt * TR, wave);
+        sv.go(base + TILE, vb + (int64_t)kt * TR * v.tok, sp.len - kt * TR, wave);
+    };
+    stage(0, 0);
+    unsigned char mb = MASK ? mask_byte(mask, sp.s0, lane, sp.len) : 0;
+    const int nloop = MASK ? nt : sp.len / TR;
+    for (int kt = 0; kt < nloop; ++kt) {
+        const int cur = (kt & 1) * SLOT;
+        unsigned long long bits = 0;
+        if constexpr (MASK) {
+            bits = __ballot(mb != 0);
+            if (wave == 0) bias[kt & 1][lane] = mb ? 0.f : -INFINITY;
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // tile kt has landed for every wave, and the other slot is read by none
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + 1 < nt) {
+            stage(SLOT - cur, kt + 1);
+            if constexpr (MASK) mb = mask_byte(mask, sp.s0, (kt + 1) * TR + lane, sp.len);
+        }
+        if constexpr (MASK) {
+            if (bits == 0) continue;  // every wave has the same bits
+            if (~bits) {
+                zero_rows<D>(smem + cur, bits);
+                zero_rows<D>(smem + cur + TILE, bits);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+            }
+        }
+        tile(std::integral_constant<bool, MASK>{}, cur, bias[kt & 1], kt == 0);
+    }
+    if (!MASK && nloop < nt) {  // rows past the end landed as zeros
+        const int cur = (nloop & 1) * SLOT;
+        if (wave == 0) bias[0][lane] = nloop * TR + lane < sp.len ? 0.f : -INFINITY;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        tile(std::true_type{}, cur, bias[0], nloop == 0);
+    }
+}
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-template <int D>
-__global__ __launch_bounds__(AG_WAVES * 64) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
+template <int D, bool MASK>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 4 : 2) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
                                                                      float* __restrict__ lse, const int* __restrict__ cu,
                                                                      int n_seg, const unsigned char* __restrict__ mask,
-                                                                     int N, int H, int group, int n_blk, int grid, float c) {
-    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+                                                                     int N, int group, Order od, float c) {
+    constexpr int TILE = TR * 2 * D;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+    __shared__ __attribute__((aligned(16))) float bias[2][TR];
     const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_remap(blockIdx.x, grid);
-    const int head = id / n_blk;
-    const Span sp = find_span(id - head * n_blk, cu, n_seg, N, 128);
-    if (sp.first >= sp.len) return;
+    int head;
+    Span sp;
+    if (!find_span(od, cu, n_seg, N, head, sp)) return;
     const int row = sp.first + wave * 32 + l31;
     const bool on = row < sp.len;
     const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
@@ -267,118 +377,93 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_fwd_lse_kernel(View q, Vie
         if (on && hi == 0) lse[(int64_t)head * N + tok] = -INFINITY;
         return;
     }
-    const __bf16* kb = k.p + sp.s0 * k.tok + (head / group) * k.head;
-    const __bf16* vb = v.p + sp.s0 * v.tok + (head / group) * v.head;
-    Stage<D> sk, sv;
-    sk.init(k.tok, wave, lane);
-    sv.init(v.tok, wave, lane);
-    const int nt = (sp.len + TR - 1) / TR;
-    auto stage = [&](int slot, int kt) {
-        char* base = smem + slot;
-        sk.go(base, kb + (int64_t)kt * TR * k.tok, sp.len - kt * TR, wave);
-        sv.go(base + TILE, vb + (int64_t)kt * TR * v.tok, sp.len - kt * TR, wave);
-    };
-    stage(0, 0);
-    unsigned char mb = mask_byte(mask, sp.s0, lane, sp.len);
     bf16x8 qf[D / 16];
     {
         const __bf16* qp = q.p + tok * q.tok + head * q.head + hi * 8;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8*)(qp + ks * 16);
     }
-    int koff[2];
-    koff[0] = row_off<D>(0, l31, hi);
-    koff[1] = row_off<D>(1, l31, hi);
+    const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
-    float m = -INFINITY, l = 0.f;  // running maximum of q.k (before the scale), this half-wave's part of the row sum
-
-    auto tile = [&](auto masked, int cur, unsigned long long bits) {
-        constexpr bool MASKED = decltype(masked)::value;
+    // p = exp2(c s - mc).  Any reference mc gives the same quotient, so it follows the row maximum only where it has to: it
+    // is taken from the first tile with keys, and again when a tile's sum passes 2^60 (fp32 sums and bf16 probabilities have
+    // the range).  That spares the maximum over every tile.
+    float mc = 0.f, l = 0.f;
+    bool fresh = true;  // no reference yet
+    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st, bool) {
+        constexpr bool BIASED = decltype(biased)::value;
         f32x16 s[2];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            s[mt] = mfma_rows<D>(smem + cur, koff[mt], qf, splat16(0.f));
-            if constexpr (MASKED) {
-                const unsigned b = (unsigned)(bits >> (32 * mt)) >> (4 * hi);
+        for (int mt = 0; mt < 2; ++mt) s[mt] = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
+        bf16x8 p[2][2];
+        float ps;
+        auto probabilities = [&] {
+            ps = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!(b & (1u << crow(r, 0)))) s[mt][r] = -INFINITY;
+            for (int mt = 0; mt < 2; ++mt) {
+                float e[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    e[r] = __builtin_amdgcn_exp2f(fmaf(s[mt][r], c, -mc));
+                    ps += e[r];
+                }
+                // 2^-8 relative at most, in the product with V only; the row sum keeps fp32
+                p[mt][0] = pack8(e);
+                p[mt][1] = pack8(e + 8);
             }
+        };
+        auto largest = [&] {
+            float mx = s[0][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[1][r]);
+            mx = half_max(mx) * c;
+            return mx == -INFINITY ? 0.f : mx;
+        };
+        if (fresh) {  // a tile with keys has them for every row
+            mc = largest();
+            fresh = false;
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[1][r]);
-        mx = half_max(mx);
-        // The reference point only follows a maximum that has outgrown it by 2^8 (any reference point gives the same
-        // quotient; fp32 sums and bf16 probabilities have the range).
-        if (__any((mx - m) * c > 8.f)) {
-            const float mn = fmaxf(m, mx);
-            const float a = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * c);
-            m = mn;
+        probabilities();
+        if (__builtin_expect(__any(!(ps <= 1.152921504606847e18f)), 0)) {
+            const float mn = fmaxf(mc, largest());
+            const float a = __builtin_amdgcn_exp2f(mc - mn);
+            mc = mn;
             l *= a;
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[t][r] *= a;
+            probabilities();
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
-        bf16x8 p[2][2];
-        float ps = 0.f;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[mt][r], c, -mc));
-                ps += e;
-                p[mt][r >> 3][r & 7] = (__bf16)e;  // 2^-9 relative, in the product with V only; the row sum keeps fp32
-            }
         l += ps;
         mfma_tr<D, 0>(acc, ta, lds0 + cur + TILE, p[0]);
         mfma_tr<D, 1>(acc, ta, lds0 + cur + TILE, p[1]);
-    };
-    for (int kt = 0; kt < nt; ++kt) {
-        const int cur = (kt & 1) * SLOT, left = sp.len - kt * TR;
-        const unsigned long long bits = __ballot(mb != 0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();  // tile kt has landed for every wave, and the other slot is read by none
-        __builtin_amdgcn_sched_barrier(0);
-        if (kt + 1 < nt) {
-            stage(SLOT - cur, kt + 1);
-            mb = mask_byte(mask, sp.s0, (kt + 1) * TR + lane, sp.len);
-        }
-        if (mask && bits != (left >= TR ? ~0ull : (1ull << left) - 1)) {  // uniform: every wave has the same bits
-            zero_rows<D>(smem + cur + TILE, bits);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-        }
-        if (bits == ~0ull) tile(std::false_type{}, cur, bits);
-        else if (bits) tile(std::true_type{}, cur, bits);
-    }
+    });
     l = half_sum(l);
-    store_row<D>(op, acc, l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l), hi, on);  // no key: zeros; NaN stays
-    if (on && hi == 0) lse[(int64_t)head * N + tok] = l == 0.f ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * AG_LN2;
+    store_row<D>(op, acc, l > 0.f ? 1.0f / l : l, hi, on);  // no key: zeros; NaN stays
+    if (on && hi == 0) lse[(int64_t)head * N + tok] = l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * AG_LN2;
 }
 
 // ---- backward: dQ and delta --------------------------------------------------------------------------------------------
-template <int D>
-__global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dq_kernel(View dout, View q, View k, View v, View o,
+template <int D, bool MASK>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_kernel(View dout, View q, View k, View v, View o,
                                                                     const float* __restrict__ lse,
                                                                     float* __restrict__ delta, OutView dq,
                                                                     const int* __restrict__ cu, int n_seg,
-                                                                    const unsigned char* __restrict__ mask, int N, int H,
-                                                                    int group, int n_blk, int grid, float scale) {
-    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
+                                                                    const unsigned char* __restrict__ mask, int N,
+                                                                    int group, Order od, float scale) {
+    constexpr int TILE = TR * 2 * D;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+    __shared__ __attribute__((aligned(16))) float bias[2][TR];
     const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_remap(blockIdx.x, grid);
-    const int head = id / n_blk;
-    const Span sp = find_span(id - head * n_blk, cu, n_seg, N, 128);
-    if (sp.first >= sp.len) return;
+    int head;
+    Span sp;
+    if (!find_span(od, cu, n_seg, N, head, sp)) return;
     const int row = sp.first + wave * 32 + l31;
     const bool on = row < sp.len;
     const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
@@ -390,19 +475,6 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dq_kernel(View dout, V
         store_row<D>(op, acc, 0.f, hi, on);
         return;
     }
-    const __bf16* kb = k.p + sp.s0 * k.tok + (head / group) * k.head;
-    const __bf16* vb = v.p + sp.s0 * v.tok + (head / group) * v.head;
-    Stage<D> sk, sv;
-    sk.init(k.tok, wave, lane);
-    sv.init(v.tok, wave, lane);
-    const int nt = (sp.len + TR - 1) / TR;
-    auto stage = [&](int slot, int kt) {
-        char* base = smem + slot;
-        sk.go(base, kb + (int64_t)kt * TR * k.tok, sp.len - kt * TR, wave);
-        sv.go(base + TILE, vb + (int64_t)kt * TR * v.tok, sp.len - kt * TR, wave);
-    };
-    stage(0, 0);
-    unsigned char mb = mask_byte(mask, sp.s0, lane, sp.len);
     bf16x8 qf[D / 16], gf[D / 16];
     float dl = 0.f;
     {
@@ -420,75 +492,52 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dq_kernel(View dout, V
     }
     dl = half_sum(dl);
     const float c = scale * AG_LOG2E;
-    const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;  // +inf for a row without keys: every key is masked there
+    const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;  // +inf only where every tile is skipped
     if (on && hi == 0) delta[(int64_t)head * N + tok] = dl;
-    int koff[2];
-    koff[0] = row_off<D>(0, l31, hi);
-    koff[1] = row_off<D>(1, l31, hi);
+    const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    const f32x16 nd = splat16(-dl);  // dP starts from -delta
 
-    auto half = [&](auto masked, auto mt_, int cur, unsigned long long bits) {
-        constexpr bool MASKED = decltype(masked)::value;
-        constexpr int mt = decltype(mt_)::value;
-        const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, splat16(0.f));
-        const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], gf, splat16(0.f));
-        bf16x8 ds[2];
-        const unsigned b = (unsigned)(bits >> (32 * mt)) >> (4 * hi);
+    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st, bool) {
+        constexpr bool BIASED = decltype(biased)::value;
+        auto half = [&](auto mt_) {
+            constexpr int mt = decltype(mt_)::value;
+            const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
+            const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], gf, nd);
+            float e[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float e = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * (dp[r] - dl);
-            if constexpr (MASKED)
-                if (!(b & (1u << crow(r, 0)))) e = 0.f;
-            ds[r >> 3][r & 7] = (__bf16)e;  // 2^-9 relative, for the product with K
-        }
-        mfma_tr<D, mt>(acc, ta, lds0 + cur, ds);
-    };
-    for (int kt = 0; kt < nt; ++kt) {
-        const int cur = (kt & 1) * SLOT, left = sp.len - kt * TR;
-        const unsigned long long bits = __ballot(mb != 0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        if (kt + 1 < nt) {
-            stage(SLOT - cur, kt + 1);
-            mb = mask_byte(mask, sp.s0, (kt + 1) * TR + lane, sp.len);
-        }
-        if (mask && bits != (left >= TR ? ~0ull : (1ull << left) - 1)) {
-            zero_rows<D>(smem + cur, bits);
-            zero_rows<D>(smem + cur + TILE, bits);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-        }
-        if (bits == ~0ull) {
-            half(std::false_type{}, std::integral_constant<int, 0>{}, cur, bits);
-            half(std::false_type{}, std::integral_constant<int, 1>{}, cur, bits);
-        } else if (bits) {
-            half(std::true_type{}, std::integral_constant<int, 0>{}, cur, bits);
-            half(std::true_type{}, std::integral_constant<int, 1>{}, cur, bits);
-        }
-    }
+            for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
+            const bf16x8 ds[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with K
+            mfma_tr<D, mt>(acc, ta, lds0 + cur, ds);
+        };
+        half(std::integral_constant<int, 0>{});
+        half(std::integral_constant<int, 1>{});
+    });
     store_row<D>(op, acc, scale, hi, on);
 }
 
 // ---- backward: dK and dV -----------------------------------------------------------------------------------------------
+// At head dim 128 the accumulators take 128 registers and K's fragments 32; V's would leave one wave per SIMD, so they are
+// read from LDS where they are used (LDS reads run at 256 bytes a cycle, a third of the time unused), and the ring holds
+// 32-row tiles: 64 KiB a workgroup, two of them on a CU.
 template <int D>
-__global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dkdv_kernel(View dout, View q, View k, View v,
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_kernel(View dout, View q, View k, View v,
                                                                       const float* __restrict__ lse,
                                                                       const float* __restrict__ delta, OutView dk,
                                                                       OutView dv, const int* __restrict__ cu, int n_seg,
-                                                                      const unsigned char* __restrict__ mask, int N, int G,
-                                                                      int group, int n_blk, int grid, float scale) {
-    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][TR];  // slot, (-lse log2 e, -delta), row of the tile
+                                                                      const unsigned char* __restrict__ mask, int N,
+                                                                      int group, Order od, float scale) {
+    constexpr bool VL = D == 128;
+    constexpr int RT = VL ? 32 : 64, TILE = RT * 2 * D, SLOT = 2 * TILE;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT + (VL ? AG_BLK * 2 * D : 0)];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][RT];  // slot, (-lse / scale, -delta), row of the tile
     const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_remap(blockIdx.x, grid);
-    const int kvh = id / n_blk;
-    const Span sp = find_span(id - kvh * n_blk, cu, n_seg, N, 128);
-    if (sp.first >= sp.len) return;
+    int kvh;
+    Span sp;
+    if (!find_span(od, cu, n_seg, N, kvh, sp)) return;
     const int row = sp.first + wave * 32 + l31;
     const bool on = row < sp.len;
     const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
@@ -503,8 +552,9 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dkdv_kernel(View dout,
         store_row<D>(ovp, av, 0.f, hi, on);
         return;
     }
-    // A key that takes no part has its own lane: its column is computed from zero rows and not used.
-    bf16x8 kf[D / 16], vf[D / 16];
+    // A key that takes no part has its own lane: its column is computed, from zero rows where its fragments are registers,
+    // and not used.
+    bf16x8 kf[D / 16], vf[VL ? 1 : D / 16];
     {
         const __bf16* kp = k.p + tok * k.tok + kvh * k.head + hi * 8;
         const __bf16* vp = v.p + tok * v.tok + kvh * v.head + hi * 8;
@@ -513,35 +563,50 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dkdv_kernel(View dout,
             u32x4 a = u32x4{0u, 0u, 0u, 0u}, b = a;
             if (live) {
                 a = *(const u32x4*)(kp + ks * 16);
-                b = *(const u32x4*)(vp + ks * 16);
+                if constexpr (!VL) b = *(const u32x4*)(vp + ks * 16);
             }
             kf[ks] = __builtin_bit_cast(bf16x8, a);
-            vf[ks] = __builtin_bit_cast(bf16x8, b);
+            if constexpr (!VL) vf[ks] = __builtin_bit_cast(bf16x8, b);
         }
     }
-    Stage<D> sq, sg;
+    if constexpr (VL) {  // the wave's own 32 rows, so that nothing but its own loads has to be waited for
+        const int r0 = sp.first + wave * 32, rows = sp.len - r0;
+        if (rows > 0) {
+            const __bf16* vb = v.p + (sp.s0 + r0) * v.tok + kvh * v.head;
+            const int nrec = (int)((rows < 32 ? rows - 1 : 31) * (unsigned)(v.tok * 2) + 2 * D);
+            const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)vb, 0, nrec, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + lane / 16;
+                const unsigned off = (unsigned)r * (unsigned)(v.tok * 2) + (unsigned)((lane & 15) ^ swz<D>(r)) * 16u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(d, LDS_PTR(smem + 2 * SLOT + wave * 32 * 2 * D + i * 1024), 16, (int)off, 0, 0, 0);
+            }
+        }
+    }
+    Stage<D, RT> sq, sg;
     sq.init(q.tok, wave, lane);
     sg.init(dout.tok, wave, lane);
-    const int nt = (sp.len + TR - 1) / TR;  // query tiles per head of the group
+    const int nt = (sp.len + RT - 1) / RT;  // query tiles per head of the group
     const int total = nt * group;
+    const float inv_scale = 1.0f / scale;
     float next = 0.f;
-    auto stage = [&](int slot, int i) {
-        const int g = i / nt, qt = i - g * nt, left = sp.len - qt * TR;
-        const int head = kvh * group + g;
-        const int64_t t0 = sp.s0 + (int64_t)qt * TR;
+    int gq = 0, qt = 0;  // head of the group and tile that stage() takes next
+    auto stage = [&](int slot) {
+        const int left = sp.len - qt * RT, head = kvh * group + gq;
+        const int64_t t0 = sp.s0 + (int64_t)qt * RT;
         char* base = smem + slot;
         sq.go(base, q.p + t0 * q.tok + head * q.head, left, wave);
         sg.go(base + TILE, dout.p + t0 * dout.tok + head * dout.head, left, wave);
         if (wave < 2) {  // wave 0: lse, wave 1: delta.  Rows past the end get probability 2^-inf = 0
             const float* src = (wave ? delta : lse) + (int64_t)head * N + t0;
-            const float x = lane < left ? src[lane] : (wave ? 0.f : INFINITY);
-            next = wave ? -x : -x * AG_LOG2E;
+            const float x = lane < left && lane < RT ? src[lane] : (wave ? 0.f : INFINITY);
+            next = wave ? -x : -x * inv_scale;
         }
+        if (++qt == nt) { qt = 0; ++gq; }
     };
-    stage(0, 0);
-    int koff[2];
-    koff[0] = row_off<D>(0, l31, hi);
-    koff[1] = row_off<D>(1, l31, hi);
+    stage(0);
+    const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
+    const int voff = 2 * SLOT + wave * 32 * 2 * D + row_off<D>(0, l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
@@ -549,34 +614,36 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dkdv_kernel(View dout,
 
     auto half = [&](auto mt_, int cur, const float* st) {
         constexpr int mt = decltype(mt_)::value;
-        f32x16 nl, nd;
+        const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], kf, rows16(st, mt, hi));  // Q K^T - lse / scale
+        f32x16 dp = rows16(st + RT, mt, hi);                                          // dO V^T - delta
+        if constexpr (VL) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 a = *(const f32x4*)(st + 32 * mt + 8 * g + 4 * hi), b = *(const f32x4*)(st + TR + 32 * mt + 8 * g + 4 * hi);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { nl[4 * g + e] = a[e]; nd[4 * g + e] = b[e]; }
+            for (int ks = 0; ks < D / 16; ++ks)
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(smem + cur + TILE + (koff[mt] ^ (ks << 5))),
+                                                             *(const bf16x8*)(smem + (voff ^ (ks << 5))), dp, 0, 0, 0);
+        } else {
+            dp = mfma_rows<D>(smem + cur + TILE, koff[mt], vf, dp);
         }
-        const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], kf, splat16(0.f));
-        const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], vf, nd);  // dO V^T - delta
-        bf16x8 p[2], ds[2];
+        float e[16], f[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl[r]));
-            p[r >> 3][r & 7] = (__bf16)e;  // 2^-9 relative, for the products with dO and Q
-            ds[r >> 3][r & 7] = (__bf16)(e * dp[r]);
+            e[r] = __builtin_amdgcn_exp2f(s[r] * c);
+            f[r] = e[r] * dp[r];
         }
+        // 2^-8 relative at most, for the products with dO and Q
+        const bf16x8 p[2] = {pack8(e), pack8(e + 8)}, ds[2] = {pack8(f), pack8(f + 8)};
         mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
         mfma_tr<D, mt>(ak, ta, lds0 + cur, ds);
     };
     for (int i = 0; i < total; ++i) {
         const int cur = (i & 1) * SLOT;
-        if (wave < 2) stat[i & 1][wave][lane] = next;
+        if (wave < 2 && lane < RT) stat[i & 1][wave][lane] = next;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 < total) stage(SLOT - cur, i + 1);
+        if (i + 1 < total) stage(SLOT - cur);
         half(std::integral_constant<int, 0>{}, cur, &stat[i & 1][0][0]);
-        half(std::integral_constant<int, 1>{}, cur, &stat[i & 1][0][0]);
+        if constexpr (RT == 64) half(std::integral_constant<int, 1>{}, cur, &stat[i & 1][0][0]);
     }
     if (!live) {
 #pragma unroll
@@ -584,6 +651,19 @@ __global__ __launch_bounds__(AG_WAVES * 64) void attn_bwd_dkdv_kernel(View dout,
     }
     store_row<D>(okp, ak, scale, hi, on);
     store_row<D>(ovp, av, 1.f, hi, on);
+}
+
+Order ag_order(int N, int n_seg, int heads) {
+    Order o;
+    o.n_blk = N / AG_BLK + n_seg + 2;
+    o.chunk = N / AG_BLK / (n_seg > 0 ? n_seg : 1) + 1;
+    o.heads = heads;
+    const int groups = (o.n_blk + o.chunk - 1) / o.chunk * heads;
+    o.grid = (groups + 31) / 32 * 32 * o.chunk;
+    o.by_chunk = 0xffffffffu / (unsigned)o.chunk;
+    o.by_heads = 0xffffffffu / (unsigned)heads;
+    o.per_blk = (float)(n_seg + 2) / (float)o.n_blk;
+    return o;
 }
 
 bool ag_strides(const void* p, const int64_t* st, int D) {
@@ -596,7 +676,7 @@ int ag_check(const char* who, const int32_t* cu, int n_seg, int N, int H, int G,
     if (N < 0 || N > (1 << 30) || n_seg < 0 || H <= 0 || G <= 0 || H % G) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: n_tokens=%d, n_segments=%d, heads=%d, kv heads=%d", who, N, n_seg, H, G);
     if (!(scale > 0.f && scale < 1e30f)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: scale must be positive and finite", who);
     if (N > 0 && !cu) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: null pointer", who);
-    if (((long long)N / 128 + n_seg + 2) * H > 0x7fffffffLL) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: grid too large", who);
+    if (2 * ((long long)N / AG_BLK + n_seg + 3) * (H + 32) > 0x7fffffffLL) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: grid too large", who);
     return ESMK_OK;
 }
 
@@ -615,10 +695,12 @@ extern "C" int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v,
             ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_fwd: tensor %d: address and strides must be multiples of 16 bytes, token stride >= head_dim", i);
     const View vq{(const __bf16*)q, strides[0], strides[1]}, vk{(const __bf16*)k, strides[2], strides[3]}, vv{(const __bf16*)v, strides[4], strides[5]};
     const OutView vo{(__bf16*)out, strides[6], strides[7]};
-    const int n_blk = n_tokens / 128 + n_segments + 2, grid = n_blk * n_heads, group = n_heads / n_kv_heads;
-    auto* kern = head_dim == 64 ? attn_fwd_lse_kernel<64> : attn_fwd_lse_kernel<128>;
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(AG_WAVES * 64), 0, (hipStream_t)stream, vq, vk, vv, vo, lse, cu_seqlens, n_segments,
-                       key_mask, n_tokens, n_heads, group, n_blk, grid, scale * AG_LOG2E);
+    const int group = n_heads / n_kv_heads;
+    const Order od = ag_order(n_tokens, n_segments, n_heads);
+    auto* kern = head_dim == 64 ? (key_mask ? attn_fwd_lse_kernel<64, true> : attn_fwd_lse_kernel<64, false>)
+                                : (key_mask ? attn_fwd_lse_kernel<128, true> : attn_fwd_lse_kernel<128, false>);
+    hipLaunchKernelGGL(kern, dim3(od.grid), dim3(AG_WAVES * 64), 0, (hipStream_t)stream, vq, vk, vv, vo, lse, cu_seqlens, n_segments,
+                       key_mask, n_tokens, group, od, scale * AG_LOG2E);
     ESMK_CHECK_LAUNCH("esmk_attn_varlen_fwd");
     return ESMK_OK;
 }
@@ -643,15 +725,17 @@ extern "C" int esmk_attn_varlen_bwd(const void* dout, const void* q, const void*
         ESMK_FAIL(ESMK_ERR_WORKSPACE, "esmk_attn_varlen_bwd: needs %zu workspace bytes", esmk_attn_varlen_bwd_workspace_bytes(n_tokens, n_heads));
     auto in = [&](int i) { return View{(const __bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
     auto ov = [&](int i) { return OutView{(__bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
-    const int n_blk = n_tokens / 128 + n_segments + 2, group = n_heads / n_kv_heads;
+    const int group = n_heads / n_kv_heads;
+    const Order oq = ag_order(n_tokens, n_segments, n_heads), ok = ag_order(n_tokens, n_segments, n_kv_heads);
     float* delta = (float*)workspace;
     hipStream_t s = (hipStream_t)stream;
-    auto* kq = head_dim == 64 ? attn_bwd_dq_kernel<64> : attn_bwd_dq_kernel<128>;
-    hipLaunchKernelGGL(kq, dim3(n_blk * n_heads), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), in(4), lse, delta, ov(5),
-                       cu_seqlens, n_segments, key_mask, n_tokens, n_heads, group, n_blk, n_blk * n_heads, scale);
+    auto* kq = head_dim == 64 ? (key_mask ? attn_bwd_dq_kernel<64, true> : attn_bwd_dq_kernel<64, false>)
+                              : (key_mask ? attn_bwd_dq_kernel<128, true> : attn_bwd_dq_kernel<128, false>);
+    hipLaunchKernelGGL(kq, dim3(oq.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), in(4), lse, delta, ov(5),
+                       cu_seqlens, n_segments, key_mask, n_tokens, group, oq, scale);
     auto* kk = head_dim == 64 ? attn_bwd_dkdv_kernel<64> : attn_bwd_dkdv_kernel<128>;
-    hipLaunchKernelGGL(kk, dim3(n_blk * n_kv_heads), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), lse, delta, ov(6), ov(7),
-                       cu_seqlens, n_segments, key_mask, n_tokens, n_kv_heads, group, n_blk, n_blk * n_kv_heads, scale);
+    hipLaunchKernelGGL(kk, dim3(ok.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), lse, delta, ov(6), ov(7),
+                       cu_seqlens, n_segments, key_mask, n_tokens, group, ok, scale);
     ESMK_CHECK_LAUNCH("esmk_attn_varlen_bwd");
     return ESMK_OK;
 }
