@@ -9,11 +9,14 @@
 // logits leaves (max, log-sum, log-probability) of every token, a workgroup per pair adds the log-probabilities (in 64
 // bits: a margin is a small difference of two long sums) and leaves c_t, and the backward pass reads the logits once more
 // and writes the gradient.  All three are bound by memory; sums run in a fixed order.
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace {
 
-// token state: max, log of the sum of exp(z - max), log-probability of the target, c_t
+// token state: max, log of the sum of exp(z - max), log-probability of the target, c_t (until the pair is known: 1 if the
+// token is scored, else 0)
 typedef f32x4 TokState;
 
 template <typename T> struct PlT;
@@ -76,29 +79,45 @@ struct Row {
     }
 };
 
+template <int CTRL>
+__device__ __forceinline__ float pl_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
 template <int LPR>
 __device__ __forceinline__ float row_max(float v) {
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    if constexpr (LPR == 64) {
+        v = fmaxf(v, __shfl_xor(v, 32));
+        v = fmaxf(v, __shfl_xor(v, 16));
+    }
+    // within 16 lanes on the vector ALU: lane ^ 1, lane ^ 2, mirrored in 8, mirrored in 16
+    v = fmaxf(v, pl_dpp<0xB1>(v));
+    v = fmaxf(v, pl_dpp<0x4E>(v));
+    v = fmaxf(v, pl_dpp<0x141>(v));
+    return fmaxf(v, pl_dpp<0x140>(v));
 }
 template <int LPR>
 __device__ __forceinline__ float row_add(float v) {
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    if constexpr (LPR == 64) {
+        v += __shfl_xor(v, 32);
+        v += __shfl_xor(v, 16);
+    }
+    v += pl_dpp<0xB1>(v);
+    v += pl_dpp<0x4E>(v);
+    v += pl_dpp<0x141>(v);
+    return v + pl_dpp<0x140>(v);
 }
 
 // LPR lanes per row
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void pref_token_kernel(const T* __restrict__ z, const int64_t* __restrict__ targets,
-                                                         TokState* __restrict__ tok, int N, int V) {
+                                                         const int* __restrict__ cu, int n_seq, TokState* __restrict__ tok,
+                                                         int N, int V) {
     constexpr int E = PlT<T>::N, CH = 4;  // pieces in flight per lane
     const int sub = threadIdx.x & (LPR - 1);
     const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
     if (row >= N) return;
     const int64_t y = targets[row];
-    if (y < 0 || y >= V) {  // not scored: its logits are not looked at
+    if (y < 0 || y >= V || row < cu[0] || row >= cu[n_seq]) {  // not scored: its logits are not looked at
         if (sub == 0) tok[row] = TokState{0.f, 0.f, 0.f, 0.f};
         return;
     }
@@ -131,66 +150,81 @@ __global__ __launch_bounds__(256) void pref_token_kernel(const T* __restrict__ z
     l = row_add<LPR>(l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * PL_LOG2E)));
     if (sub == 0) {
         const float ls = logf(l);  // no finite logit: log 0, and the row's loss is not finite, as the formula has it
-        tok[row] = TokState{top, ls, (pl_get(z + row * V + y) - top) - ls, 0.f};
+        tok[row] = TokState{top, ls, (pl_get(z + row * V + y) - top) - ls, 1.f};
     }
 }
 
-// one workgroup per pair
-__global__ __launch_bounds__(256) void pref_pair_kernel(const int64_t* __restrict__ targets, TokState* __restrict__ tok,
-                                                        const int* __restrict__ cu, const float* __restrict__ ref, int N,
-                                                        int V, int P, double beta, double eps, double alpha,
-                                                        float* __restrict__ logps, double* __restrict__ pair_loss,
-                                                        float* __restrict__ loss) {
-    __shared__ double red[2][4];
-    __shared__ int cnt[4];
+// One workgroup per pair: a few dependent reads long, so a thread requests up to four tokens of both sequences at once.
+constexpr int PL_PAIR = 512;
+__global__ __launch_bounds__(PL_PAIR) void pref_pair_kernel(TokState* __restrict__ tok, const int* __restrict__ cu,
+                                                            const float* __restrict__ ref, int N, int P, double beta,
+                                                            double eps, double alpha, float* __restrict__ logps,
+                                                            double* __restrict__ pair_loss, float* __restrict__ loss) {
+    constexpr int WAVES = PL_PAIR / 64, AHEAD = 4;
+    __shared__ double red[2][WAVES];
+    __shared__ int cnt[WAVES];
     const int i = blockIdx.x, wave = threadIdx.x >> 6;
-    int lo[2], hi[2], scored = 0;
-    double l[2];
+    const int at[3] = {min(max(cu[2 * i], 0), N), min(max(cu[2 * i + 1], 0), N), min(max(cu[2 * i + 2], 0), N)};
+    const f32x2 r = {ref[2 * i], ref[2 * i + 1]};
+    double a[2] = {0.0, 0.0};
+    int n = 0;
+    for (int t0 = threadIdx.x; at[0] + t0 < at[1] || at[1] + t0 < at[2]; t0 += PL_PAIR * AHEAD) {
+        f32x2 v[2][AHEAD];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        lo[s] = min(max(cu[2 * i + s], 0), N);
-        hi[s] = min(max(cu[2 * i + s + 1], lo[s]), N);
-        double a = 0.0;
-        int n = 0;
-        for (int t = lo[s] + (int)threadIdx.x; t < hi[s]; t += 256) {
-            const int64_t y = targets[t];
-            if (y >= 0 && y < V) {
-                a += (double)tok[t][2];
-                ++n;
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int t = at[s] + t0 + j * PL_PAIR;
+                v[s][j] = t < at[s + 1] ? *((const f32x2*)(tok + t) + 1) : f32x2{0.f, 0.f};
             }
-        }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o); n += __shfl_xor(n, o); }
-        if ((threadIdx.x & 63) == 0) {
-            red[s][wave] = a;
-            if (s == 0) cnt[wave] = n;
-        }
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                a[s] += (double)v[s][j][0];  // 0 where the token is not scored
+                if (s == 0) n += v[s][j][1] != 0.f;
+            }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        a[0] += __shfl_xor(a[0], o);
+        a[1] += __shfl_xor(a[1], o);
+        n += __shfl_xor(n, o);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        red[0][wave] = a[0];
+        red[1][wave] = a[1];
+        cnt[wave] = n;
     }
     __syncthreads();
+    double l[2] = {0.0, 0.0};
+    int scored = 0;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) l[s] = (red[s][0] + red[s][1]) + (red[s][2] + red[s][3]);
-    scored = max(1, cnt[0] + cnt[1] + cnt[2] + cnt[3]);
-    const double m = beta * ((l[0] - (double)ref[2 * i]) - (l[1] - (double)ref[2 * i + 1]));
-    const double t = exp(-fabs(m)), up = m >= 0.0 ? 1.0 / (1.0 + t) : t / (1.0 + t), down = m >= 0.0 ? t / (1.0 + t) : 1.0 / (1.0 + t);
-    const double lg = log1p(t), sp = fmax(m, 0.0) + lg, sn = fmax(-m, 0.0) + lg;
-    // a term whose weight is zero is left out: 0 x inf would be NaN
-    double L = eps != 1.0 ? (1.0 - eps) * sn : 0.0;
-    if (eps != 0.0) L += eps * sp;
-    if (alpha != 0.0) L -= alpha * l[0] / scored;
+    for (int w = 0; w < WAVES; ++w) {
+        l[0] += red[0][w];
+        l[1] += red[1][w];
+        scored += cnt[w];
+    }
+    scored = max(1, scored);
+    const double m = beta * ((l[0] - (double)r[0]) - (l[1] - (double)r[1]));
+    const double t = exp(-fabs(m)), q = 1.0 / (1.0 + t), up = m >= 0.0 ? q : t * q, down = m >= 0.0 ? t * q : q;
     const double gm = beta * (eps * up - (1.0 - eps) * down) / P;
     const float c[2] = {(float)(gm - alpha / scored / P), (float)-gm};
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+        for (int k = at[s] + (int)threadIdx.x; k < at[s + 1]; k += PL_PAIR)
+            if (tok[k][3] != 0.f) tok[k][3] = c[s];
     if (threadIdx.x == 0) {
+        const double lg = log1p(t), sp = fmax(m, 0.0) + lg, sn = fmax(-m, 0.0) + lg;
+        // a term whose weight is zero is left out: 0 x inf would be NaN
+        double L = eps != 1.0 ? (1.0 - eps) * sn : 0.0;
+        if (eps != 0.0) L += eps * sp;
+        if (alpha != 0.0) L -= alpha * l[0] / scored;
         logps[2 * i] = (float)l[0];
         logps[2 * i + 1] = (float)l[1];
         if (P == 1) *loss = (float)L;
         else pair_loss[i] = L;
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-        for (int k = lo[s] + (int)threadIdx.x; k < hi[s]; k += 256) {
-            const int64_t y = targets[k];
-            if (y >= 0 && y < V) tok[k][3] = c[s];
-        }
 }
 
 __global__ __launch_bounds__(256) void pref_mean_kernel(const double* __restrict__ pair_loss, int P, float* __restrict__ loss) {
@@ -251,10 +285,10 @@ void pl_dispatch(int V, F f) {
 }
 
 template <typename T>
-void pl_token(const void* z, const int64_t* y, TokState* tok, int N, int V, hipStream_t s) {
+void pl_token(const void* z, const int64_t* y, const int* cu, int n_seq, TokState* tok, int N, int V, hipStream_t s) {
     pl_dispatch(V, [&](auto lpr) {
         constexpr int LPR = decltype(lpr)::value;
-        hipLaunchKernelGGL((pref_token_kernel<T, LPR>), dim3((N + 256 / LPR - 1) / (256 / LPR)), dim3(256), 0, s, (const T*)z, y, tok, N, V);
+        hipLaunchKernelGGL((pref_token_kernel<T, LPR>), dim3((N + 256 / LPR - 1) / (256 / LPR)), dim3(256), 0, s, (const T*)z, y, cu, n_seq, tok, N, V);
     });
 }
 template <typename T>
@@ -284,7 +318,7 @@ extern "C" int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* 
                                   int N, int V, void* saved, size_t saved_bytes, float* logps, float* loss,
                                   esmk_stream_t stream) {
     if (int rc = pl_check("esmk_pref_loss_fwd", logits, dtype, targets, saved, N, V)) return rc;
-    if (n_pairs <= 0) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: n_pairs=%d", n_pairs);
+    if (n_pairs <= 0 || n_pairs > (1 << 29)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: n_pairs=%d", n_pairs);
     if (!cu_seqlens || !ref_logps || !logps || !loss || !saved) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: null pointer");
     if (!(label_smoothing >= 0.0 && label_smoothing <= 1.0)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: label_smoothing outside [0, 1]");
     if (saved_bytes < esmk_pref_loss_saved_bytes(N, n_pairs))
@@ -293,10 +327,10 @@ extern "C" int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* 
     TokState* tok = (TokState*)saved;
     double* pair_loss = (double*)(tok + N);
     if (N > 0) {
-        if (dtype == ESMK_F32) pl_token<float>(logits, targets, tok, N, V, s);
-        else pl_token<__bf16>(logits, targets, tok, N, V, s);
+        if (dtype == ESMK_F32) pl_token<float>(logits, targets, cu_seqlens, 2 * n_pairs, tok, N, V, s);
+        else pl_token<__bf16>(logits, targets, cu_seqlens, 2 * n_pairs, tok, N, V, s);
     }
-    hipLaunchKernelGGL(pref_pair_kernel, dim3(n_pairs), dim3(256), 0, s, targets, tok, cu_seqlens, ref_logps, N, V, n_pairs,
+    hipLaunchKernelGGL(pref_pair_kernel, dim3(n_pairs), dim3(PL_PAIR), 0, s, tok, cu_seqlens, ref_logps, N, n_pairs,
                        beta, label_smoothing, nll_weight, logps, pair_loss, loss);
     if (n_pairs > 1) hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(256), 0, s, pair_loss, n_pairs, loss);
     ESMK_CHECK_LAUNCH("esmk_pref_loss_fwd");

@@ -592,6 +592,6 @@ def test_refusals_name_the_argument():
             (ValueError, lambda: t.preference_loss_forward(z, y, cp, ref[:1])),
             (ValueError, lambda: t.preference_loss_forward(z, y, cp, ref, label_smoothing=1.5)),
             (TypeError, lambda: t.preference_loss_forward(z, y.int(), cp, ref)),
-            (ValueError, lambda: t.preference_loss_backward(z, y, torch.zeros(8, dtype=torch.uint8, device="cuda")))):
+            (ValueError, lambda: t.preference_loss_backward(z, y, torch.zeros(8, device="cuda")))):
         with pytest.raises(err):
             call()

@@ -58,7 +58,8 @@ def test_attention_entry_points_refuse():
     refused(fwd(st=(128, 64, 128, 64, 128, 60, 128, 64)), INVALID, "tensor 2")
     refused(fwd(st=(128, 64, 128, 64, 128, 64, 56, 64)), INVALID, "tensor 3")
     refused(fwd(st=(1 << 23, 64, 128, 64, 128, 64, 128, 64)), INVALID, "tensor 0")
-    refused(fwd(N=2 ** 31 - 1, H=1024, G=1024), UNSUPPORTED, "grid")
+    refused(fwd(N=2 ** 30, H=1024, G=1024), UNSUPPORTED, "grid")
+    refused(fwd(N=2 ** 30 + 1), INVALID, "n_tokens")
     assert fwd(N=0, q=None) == 0
 
     def bwd(st=(128, 64) * 8, ws=P, nb=1 << 20, dq=P):
