@@ -65,6 +65,18 @@ struct Stage {
             off[i] = (unsigned)r * ldb + (unsigned)((lane & (CPR - 1)) ^ swz<D>(r)) * 16u;
         }
     }
+    // Rows whose bit is clear are addressed out of range and land as zeros (a masked row may hold NaN or inf, and 0 times
+    // those is NaN).
+    __device__ __forceinline__ void go_masked(char* lds, const __bf16* first, int rows, int wave, int lane, unsigned long long bits) const {
+        const int nrec = (int)((rows < ROWS ? rows - 1 : ROWS - 1) * ldb + RB);
+        const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, nrec, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = (wave * PIECES + i) * (64 / CPR) + lane / CPR;
+            const int o = (bits >> r) & 1 ? (int)off[i] : 0x7ffffff0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(d, LDS_PTR(lds + (wave * PIECES + i) * 1024), 16, o, 0, 0, 0);
+        }
+    }
     // first: first row of the tile (wave-uniform), rows: rows of it that exist (>= 1)
     __device__ __forceinline__ void go(char* lds, const __bf16* first, int rows, int wave) const {
         const int nrec = (int)((rows < ROWS ? rows - 1 : ROWS - 1) * ldb + RB);
@@ -271,14 +283,6 @@ __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict
 __device__ __forceinline__ unsigned char mask_byte(const unsigned char* mask, int64_t s0, int row, int len) {
     return row < len ? (mask ? mask[s0 + row] : 1) : 0;
 }
-// Zero the rows of a landed tile whose bit is clear (a masked row may hold NaN or inf, and 0 times those is NaN).
-template <int D>
-__device__ __forceinline__ void zero_rows(char* tile, unsigned long long bits) {
-    const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
-    if (!((bits >> r) & 1))
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) *(u32x4*)(tile + r * 2 * D + part * (D / 2) + i * 16) = u32x4{0u, 0u, 0u, 0u};
-}
 // Accumulator start of 32 scores from a row of 64 floats in LDS (0, or -inf where the key takes no part): masking costs
 // the row reads and no vector instruction.
 __device__ __forceinline__ f32x16 rows16(const float* st, int mt, int hi) {
@@ -308,38 +312,41 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
     sk.init(k.tok, wave, lane);
     sv.init(v.tok, wave, lane);
     const int nt = (sp.len + TR - 1) / TR;
-    auto stage = [&](int slot, int kt) {
+    auto stage = [&](int slot, int kt, unsigned long long bits) {
         char* base = smem + slot;
-        sk.go(base, kb + (int64_t)kt * TR * k.tok, sp.len - kt * TR, wave);
-        sv.go(base + TILE, vb + (int64_t)kt * TR * v.tok, sp.len - kt * TR, wave);
+        const __bf16 *kp = kb + (int64_t)kt * TR * k.tok, *vp = vb + (int64_t)kt * TR * v.tok;
+        if constexpr (MASK) {
+            sk.go_masked(base, kp, sp.len - kt * TR, wave, lane, bits);
+            sv.go_masked(base + TILE, vp, sp.len - kt * TR, wave, lane, bits);
+        } else {
+            sk.go(base, kp, sp.len - kt * TR, wave);
+            sv.go(base + TILE, vp, sp.len - kt * TR, wave);
+        }
     };
-    stage(0, 0);
-    unsigned char mb = MASK ? mask_byte(mask, sp.s0, lane, sp.len) : 0;
+    unsigned long long bits = 0;  // of tile kt
+    unsigned char mb = 0;         // of tile kt + 1
+    if constexpr (MASK) {
+        bits = __ballot(mask_byte(mask, sp.s0, lane, sp.len) != 0);
+        mb = mask_byte(mask, sp.s0, TR + lane, sp.len);
+    }
+    stage(0, 0, bits);
     const int nloop = MASK ? nt : sp.len / TR;
     for (int kt = 0; kt < nloop; ++kt) {
         const int cur = (kt & 1) * SLOT;
-        unsigned long long bits = 0;
-        if constexpr (MASK) {
-            bits = __ballot(mb != 0);
-            if (wave == 0) bias[kt & 1][lane] = mb ? 0.f : -INFINITY;
-        }
+        if constexpr (MASK)
+            if (wave == 0) bias[kt & 1][lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();  // tile kt has landed for every wave, and the other slot is read by none
         __builtin_amdgcn_sched_barrier(0);
-        if (kt + 1 < nt) {
-            stage(SLOT - cur, kt + 1);
-            if constexpr (MASK) mb = mask_byte(mask, sp.s0, (kt + 1) * TR + lane, sp.len);
-        }
+        const unsigned long long now = bits;
         if constexpr (MASK) {
-            if (bits == 0) continue;  // every wave has the same bits
-            if (~bits) {
-                zero_rows<D>(smem + cur, bits);
-                zero_rows<D>(smem + cur + TILE, bits);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-            }
+            bits = __ballot(mb != 0);
+            mb = mask_byte(mask, sp.s0, (kt + 2) * TR + lane, sp.len);
         }
-        tile(std::integral_constant<bool, MASK>{}, cur, bias[kt & 1], kt == 0);
+        if (kt + 1 < nt) stage(SLOT - cur, kt + 1, bits);
+        if constexpr (MASK)
+            if (now == 0) continue;  // every wave has the same bits
+        tile(std::integral_constant<bool, MASK>{}, cur, bias[kt & 1]);
     }
     if (!MASK && nloop < nt) {  // rows past the end landed as zeros
         const int cur = (nloop & 1) * SLOT;
@@ -347,13 +354,13 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        tile(std::true_type{}, cur, bias[0], nloop == 0);
+        tile(std::true_type{}, cur, bias[0]);
     }
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
 template <int D, bool MASK>
-__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 4 : 2) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
                                                                      float* __restrict__ lse, const int* __restrict__ cu,
                                                                      int n_seg, const unsigned char* __restrict__ mask,
                                                                      int N, int group, Order od, float c) {
@@ -392,7 +399,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 4 : 2) void attn_fwd_lse_k
     // the range).  That spares the maximum over every tile.
     float mc = 0.f, l = 0.f;
     bool fresh = true;  // no reference yet
-    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st, bool) {
+    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
         f32x16 s[2];
 #pragma unroll
@@ -500,7 +507,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
     const f32x16 nd = splat16(-dl);  // dP starts from -delta
 
-    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st, bool) {
+    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
         auto half = [&](auto mt_) {
             constexpr int mt = decltype(mt_)::value;
