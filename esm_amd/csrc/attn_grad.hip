@@ -217,7 +217,7 @@ __device__ __forceinline__ void store_row(__bf16* row, const f32x16 (&o)[D / 32]
 // the next) are dealt to the eight XCDs in turn.  A group shares its keys in one XCD's L2, the XCDs together read whole rows
 // of a fused qkv buffer, and sequences of unequal length load all XCDs alike.  Within an XCD four groups advance together:
 // its workgroups go to its shader engines in turn, and a group's block numbers without rows would otherwise fall to the same
-// engines every time (128-token sequences: every second number; forward pass 118 -> 72 us).
+// engines every time (128-token sequences: every second number; forward pass 118 -> 86 us).
 constexpr int AG_BLK = 128;  // rows a workgroup owns
 struct Order {
     int n_blk, chunk, heads, grid;       // chunk: block numbers of an average sequence
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void a
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
     // p = exp2(c s - mc).  Any reference mc gives the same quotient, so it follows the row maximum only where it has to: it
-    // is taken from the first tile with keys, and again when a tile's sum passes 2^60 (fp32 sums and bf16 probabilities have
+    // is taken from the first tile with keys, and again when a tile's sum passes 2^16 (fp32 sums and bf16 probabilities have
     // the range).  That spares the maximum over every tile.
     float mc = 0.f, l = 0.f;
     bool fresh = true;  // no reference yet
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void a
             fresh = false;
         }
         probabilities();
-        if (__builtin_expect(__any(!(ps <= 1.152921504606847e18f)), 0)) {
+        if (__builtin_expect(__any(!(ps <= 65536.f)), 0)) {
             const float mn = fmaxf(mc, largest());
             const float a = __builtin_amdgcn_exp2f(mc - mn);
             mc = mn;
@@ -681,9 +681,10 @@ bool ag_strides(const void* p, const int64_t* st, int D) {
 int ag_check(const char* who, const int32_t* cu, int n_seg, int N, int H, int G, int D, float scale) {
     if (D != 64 && D != 128) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: head dim %d (64 or 128)", who, D);
     if (N < 0 || N > (1 << 30) || n_seg < 0 || H <= 0 || G <= 0 || H % G) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: n_tokens=%d, n_segments=%d, heads=%d, kv heads=%d", who, N, n_seg, H, G);
-    if (!(scale > 0.f && scale < 1e30f)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: scale must be positive and finite", who);
+    if (!(scale > 1e-30f && scale < 1e30f)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: scale must be positive and finite (1e-30 .. 1e30)", who);
     if (N > 0 && !cu) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: null pointer", who);
-    if (2 * ((long long)N / AG_BLK + n_seg + 3) * (H + 32) > 0x7fffffffLL) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: grid too large", who);
+    // a launch holds fewer than 2^32 threads; the order of the blocks pads the grid to at most twice this
+    if (2 * ((long long)N / AG_BLK + n_seg + 3) * (H + 32) >= (1LL << 24)) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: grid too large", who);
     return ESMK_OK;
 }
 

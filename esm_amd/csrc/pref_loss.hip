@@ -111,8 +111,9 @@ __device__ __forceinline__ float row_add(float v) {
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void pref_token_kernel(const T* __restrict__ z, const int64_t* __restrict__ targets,
                                                          const int* __restrict__ cu, int n_seq, TokState* __restrict__ tok,
-                                                         int N, int V) {
+                                                         unsigned* __restrict__ done, int N, int V) {
     constexpr int E = PlT<T>::N, CH = 4;  // pieces in flight per lane
+    if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;  // for the pair kernel behind this one
     const int sub = threadIdx.x & (LPR - 1);
     const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
     if (row >= N) return;
@@ -159,10 +160,12 @@ constexpr int PL_PAIR = 512;
 __global__ __launch_bounds__(PL_PAIR) void pref_pair_kernel(TokState* __restrict__ tok, const int* __restrict__ cu,
                                                             const float* __restrict__ ref, int N, int P, double beta,
                                                             double eps, double alpha, float* __restrict__ logps,
-                                                            double* __restrict__ pair_loss, float* __restrict__ loss) {
+                                                            double* __restrict__ pair_loss, unsigned* __restrict__ done,
+                                                            float* __restrict__ loss) {
     constexpr int WAVES = PL_PAIR / 64, AHEAD = 4;
     __shared__ double red[2][WAVES];
     __shared__ int cnt[WAVES];
+    __shared__ bool last;
     const int i = blockIdx.x, wave = threadIdx.x >> 6;
     const int at[3] = {min(max(cu[2 * i], 0), N), min(max(cu[2 * i + 1], 0), N), min(max(cu[2 * i + 2], 0), N)};
     const f32x2 r = {ref[2 * i], ref[2 * i + 1]};
@@ -222,20 +225,24 @@ __global__ __launch_bounds__(PL_PAIR) void pref_pair_kernel(TokState* __restrict
         if (alpha != 0.0) L -= alpha * l[0] / scored;
         logps[2 * i] = (float)l[0];
         logps[2 * i + 1] = (float)l[1];
-        if (P == 1) *loss = (float)L;
-        else pair_loss[i] = L;
+        // The workgroup that finishes last adds the pairs' losses, in their order: its counter says that all are written.
+        __hip_atomic_store(pair_loss + i, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)P - 1u;
     }
-}
-
-__global__ __launch_bounds__(256) void pref_mean_kernel(const double* __restrict__ pair_loss, int P, float* __restrict__ loss) {
-    __shared__ double red[4];
-    double a = 0.0;
-    for (int i = threadIdx.x; i < P; i += 256) a += pair_loss[i];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    if (threadIdx.x == 0) *loss = (float)(((red[0] + red[1]) + (red[2] + red[3])) / P);
+    if (!last) return;
+    double sum = 0.0;
+    for (int k = threadIdx.x; k < P; k += PL_PAIR) sum += __hip_atomic_load(pair_loss + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 63) == 0) red[0][wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) sum += red[0][w];
+        *loss = (float)(sum / P);
+    }
 }
 
 template <typename T, int LPR>
@@ -285,10 +292,10 @@ void pl_dispatch(int V, F f) {
 }
 
 template <typename T>
-void pl_token(const void* z, const int64_t* y, const int* cu, int n_seq, TokState* tok, int N, int V, hipStream_t s) {
+void pl_token(const void* z, const int64_t* y, const int* cu, int n_seq, TokState* tok, unsigned* done, int N, int V, hipStream_t s) {
     pl_dispatch(V, [&](auto lpr) {
         constexpr int LPR = decltype(lpr)::value;
-        hipLaunchKernelGGL((pref_token_kernel<T, LPR>), dim3((N + 256 / LPR - 1) / (256 / LPR)), dim3(256), 0, s, (const T*)z, y, cu, n_seq, tok, N, V);
+        hipLaunchKernelGGL((pref_token_kernel<T, LPR>), dim3(N ? (N + 256 / LPR - 1) / (256 / LPR) : 1), dim3(256), 0, s, (const T*)z, y, cu, n_seq, tok, done, N, V);
     });
 }
 template <typename T>
@@ -302,6 +309,7 @@ void pl_grad(const void* z, const int64_t* y, const TokState* tok, const float* 
 int pl_check(const char* who, const void* z, int dtype, const void* targets, const void* saved, int N, int V) {
     if (N < 0 || V <= 0 || V > (1 << 30)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: N=%d, V=%d", who, N, V);
     if (dtype != ESMK_F32 && dtype != ESMK_BF16) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: bad dtype %d", who, dtype);
+    if (N >= (1 << 26)) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "%s: N=%d (at most 2^26 - 1 tokens)", who, N);  // 2^32 threads, 64 a token
     if (N > 0 && (!z || !targets || !saved)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: null pointer", who);
     if (((uintptr_t)z | (uintptr_t)saved) & 15) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "%s: logits and saved must be 16-byte aligned", who);
     return ESMK_OK;
@@ -310,7 +318,7 @@ int pl_check(const char* who, const void* z, int dtype, const void* targets, con
 }  // namespace
 
 extern "C" size_t esmk_pref_loss_saved_bytes(int N, int n_pairs) {
-    return N < 0 || n_pairs < 0 ? 0 : (size_t)N * sizeof(TokState) + (size_t)n_pairs * sizeof(double);
+    return N < 0 || n_pairs < 0 ? 0 : (size_t)N * sizeof(TokState) + (size_t)(n_pairs + 1) * sizeof(double);
 }
 
 extern "C" int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* targets, const int32_t* cu_seqlens,
@@ -326,13 +334,11 @@ extern "C" int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* 
     hipStream_t s = (hipStream_t)stream;
     TokState* tok = (TokState*)saved;
     double* pair_loss = (double*)(tok + N);
-    if (N > 0) {
-        if (dtype == ESMK_F32) pl_token<float>(logits, targets, cu_seqlens, 2 * n_pairs, tok, N, V, s);
-        else pl_token<__bf16>(logits, targets, cu_seqlens, 2 * n_pairs, tok, N, V, s);
-    }
-    hipLaunchKernelGGL(pref_pair_kernel, dim3(n_pairs), dim3(PL_PAIR), 0, s, tok, cu_seqlens, ref_logps, N, n_pairs,
-                       beta, label_smoothing, nll_weight, logps, pair_loss, loss);
-    if (n_pairs > 1) hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(256), 0, s, pair_loss, n_pairs, loss);
+    unsigned* done = (unsigned*)(pair_loss + n_pairs);
+    if (dtype == ESMK_F32) pl_token<float>(logits, targets, cu_seqlens, 2 * n_pairs, tok, done, N, V, s);
+    else pl_token<__bf16>(logits, targets, cu_seqlens, 2 * n_pairs, tok, done, N, V, s);
+    hipLaunchKernelGGL(pref_pair_kernel, dim3(n_pairs), dim3(PL_PAIR), 0, s, tok, cu_seqlens, ref_logps, N, n_pairs, beta,
+                       label_smoothing, nll_weight, logps, pair_loss, done, loss);
     ESMK_CHECK_LAUNCH("esmk_pref_loss_fwd");
     return ESMK_OK;
 }

@@ -26,7 +26,7 @@ _F32, _BF16, _I32, _I64, _U8 = (torch.float32,), (torch.bfloat16,), (torch.int32
 _MASK = (torch.bool, torch.uint8)
 _INT_MAX = 2 ** 31 - 1
 _Strides8, _Strides16 = C.c_int64 * 8, C.c_int64 * 16
-Tensor = torch.Tensor
+Tensor, _DENSE = torch.Tensor, torch.contiguous_format
 
 
 def _need(t, name, dtypes, gpu=None):
@@ -95,7 +95,7 @@ def layer_norm_forward(x, weight, bias=None, eps: float = 1e-5):
     gpu, shape, M, d = _check_norm(x, weight, bias)
     xr, ld = _rows(x, d)
     w, b = _param(weight), None if bias is None else _param(bias)
-    y, stats = x.new_empty(shape), w.new_empty((M, 2))
+    y, stats = torch.empty_like(x, memory_format=_DENSE), w.new_empty((M, 2))
     _call(gpu, "esmk_layernorm_fwd", xr.data_ptr(), _DTYPES[x.dtype], ld, w.data_ptr(), None if b is None else b.data_ptr(),
           y.data_ptr(), stats.data_ptr(), M, d, eps)
     return y, stats
@@ -112,7 +112,7 @@ def layer_norm_backward(dy, x, weight, stats, bias: bool = True, param_grads: bo
     xr, ldx = _rows(x, d)
     gr, ldg = _rows(dy, d)
     w = _param(weight)
-    dx = x.new_empty(shape)
+    dx = torch.empty_like(x, memory_format=_DENSE)
     dw = w.new_empty(d) if param_grads else None
     db = w.new_empty(d) if param_grads and bias else None
     nbytes = L.lib().esmk_layernorm_bwd_workspace_bytes(M, d) if param_grads else 0
@@ -190,8 +190,8 @@ def _check_attention(q, k, v, cu_seqlens, key_mask):
 
 def _scale(scale, D):
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 1e-30 < scale < 1e30:
+        raise ValueError(f"scale must be positive and finite (1e-30 .. 1e30), got {scale}")
     return scale
 
 
@@ -208,7 +208,7 @@ def attention_varlen_forward(q, k, v, cu_seqlens, scale: float | None = None, ke
     gpu, N, H, G, D = _check_attention(q, k, v, cu_seqlens, key_mask)
     scale = _scale(scale, D)
     (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _strided(q, "q"), _strided(k, "k"), _strided(v, "v")
-    out = q.new_empty((N, H, D))
+    out = torch.empty_like(q, memory_format=_DENSE)
     lse = q.new_empty((H, N), dtype=torch.float32)
     _call(gpu, "esmk_attn_varlen_fwd", qp, kp, vp, out.data_ptr(), lse.data_ptr(),
           _Strides8(qt, qh, kt, kh, vt, vh, H * D, D), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1,
@@ -232,7 +232,7 @@ def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float 
     dout, gp, gt, gh = _strided(dout, "dout")
     (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _strided(q, "q"), _strided(k, "k"), _strided(v, "v")
     out, op, ot, oh = _strided(out, "out")
-    dq, dk, dv = q.new_empty((N, H, D)), q.new_empty((N, G, D)), q.new_empty((N, G, D))
+    dq, dk, dv = (torch.empty_like(t, memory_format=_DENSE) for t in (q, k, v))
     nbytes = L.lib().esmk_attn_varlen_bwd_workspace_bytes(N, H)
     ws = lse.new_empty(nbytes // 4)
     _call(gpu, "esmk_attn_varlen_bwd", gp, qp, kp, vp, op, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
@@ -269,7 +269,7 @@ def _check_preference(logits, targets):
     _need(targets, "targets", _I64, gpu)
     if len(shape) != 2 or shape[1] < 1 or targets.shape != shape[:1]:
         raise ValueError(f"logits [N, V] and targets [N]: got {tuple(shape)}, {tuple(targets.shape)}")
-    if shape[0] > _INT_MAX or shape[1] > 2 ** 30:
+    if shape[0] >= 2 ** 26 or shape[1] > 2 ** 30:
         raise ValueError("logits are too large")
     return gpu, shape[0], shape[1]
 
@@ -322,7 +322,7 @@ def preference_loss_backward(logits, targets, saved, grad_loss=None):
         if grad_loss.numel() != 1:
             raise ValueError("grad_loss must be one value")
     z, y = _dense16(logits), targets.contiguous()
-    dz = z.new_empty((N, V))
+    dz = torch.empty_like(z)
     _call(gpu, "esmk_pref_loss_bwd", z.data_ptr(), _DTYPES[z.dtype], y.data_ptr(), saved.data_ptr(),
           None if grad_loss is None else grad_loss.data_ptr(), dz.data_ptr(), N, V)
     return dz

@@ -271,7 +271,7 @@ int esmk_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * token strides >= head_dim and below 2^23.  k and v have n_kv_heads heads, which divides n_heads: query head h reads key
  * head h / (n_heads / n_kv_heads).  key_mask uint8 [n_tokens] or NULL: keys whose byte is 0 take no part, whatever they hold
  * (the token's own query does).  A query without any key gets out = 0, lse = -inf; tokens in no sequence likewise.
- * scale > 0; n_tokens <= 2^30. */
+ * 1e-30 < scale < 1e30; (n_tokens / 128 + n_segments + 3) (n_heads + 32) < 2^23. */
 int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int64_t* strides,
                          const int32_t* cu_seqlens, int n_segments, const uint8_t* key_mask, int n_tokens, int n_heads,
                          int n_kv_heads, int head_dim, float scale, esmk_stream_t stream);
@@ -289,7 +289,7 @@ int esmk_attn_varlen_bwd(const void* dout, const void* q, const void* k, const v
  *   logps[s] = sum of log softmax(logits[t])[targets[t]] over the scored tokens of sequence s
  *   m_i      = beta ((logps[2i] - ref_logps[2i]) - (logps[2i+1] - ref_logps[2i+1]))
  *   loss     = mean_i [(1 - e) softplus(-m_i) + e softplus(m_i) - nll_weight logps[2i] / max(1, scored tokens of 2i)]
- * with e = label_smoothing in [0, 1].  A token is scored if 0 <= targets[t] < V; other tokens, and tokens behind the last
+ * with e = label_smoothing in [0, 1] and N < 2^26.  A token is scored if 0 <= targets[t] < V; other tokens, and tokens behind the last
  * sequence, are skipped whatever their logits hold, and get a zero gradient.  logits [N, V] dense, F32 or BF16; targets
  * int64 [N]; cu_seqlens int32 [2 n_pairs + 1] (device; clamped as above); ref_logps, logps f32 [2 n_pairs]; loss f32 [1].
  * saved: esmk_pref_loss_saved_bytes, 16-byte aligned, for the backward call. */

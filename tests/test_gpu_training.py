@@ -9,7 +9,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-U = 2.0 ** -24
+U, TINY = 2.0 ** -24, 2.0 ** -126
 R = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
 
 
@@ -161,7 +161,8 @@ def test_layer_norm_autograd_and_differences():
 def attention_oracle(q, k, v, cu, scale, mask, dout):
     """64-bit (out, lse, dq, dk, dv) and bounds.  Where the kernels round: P to bf16 before P V and P^T dO (r), dS to bf16
     before dS K and dS^T Q (r), outputs (r); delta uses the rounded out.  fp32: a score has D products (D u of their
-    magnitudes) and moves P by that, relatively; sums over keys or queries L u."""
+    magnitudes) and moves P by that, relatively; sums over keys or queries L u.  Below the smallest normal number, 2^-126, a
+    probability or a result may be flushed to zero: that much is added wherever one enters."""
     r = R[torch.bfloat16]
     N, H, D = q.shape
     G = k.shape[1]
@@ -186,13 +187,13 @@ def attention_oracle(q, k, v, cu, scale, mask, dout):
             eS = (D + 8) * U * scale * (Q.abs() @ K.abs().t()) + 4 * U * (S.abs() + ls.abs())  # abs, both S and S - lse
             eP = 2 * eS.amax(-1, keepdim=True) + (L + 32) * U                                  # rel. of P
             A = P @ V.abs()
-            tO = (r + eP) * A * (1 + r) + r * O.abs() + eP * O.abs()
+            tO = (r + eP) * A * (1 + r) + r * O.abs() + eP * O.abs() + TINY * (1 + V.abs().sum(0) + L * O.abs())
             dP = dO @ V.t()
             dl = (dO * O).sum(-1, keepdim=True)
             dS = P * (dP - dl)
             eDl = (dO.abs() * tO).sum(-1, keepdim=True) + (D + 8) * U * (dO * O).abs().sum(-1, keepdim=True)
             eDP = (D + 8) * U * (dO.abs() @ V.abs().t())
-            eds = P * (eDl + eDP + eP * (dP - dl).abs()) * (1 + r) + r * dS.abs()              # abs, of the rounded dS
+            eds = P * (eDl + eDP + eP * (dP - dl).abs()) * (1 + r) + r * dS.abs() + TINY * (1 + (dP - dl).abs())  # abs, of the rounded dS
             n = (L + 32) * U
             o[a:e, h], to[a:e, h] = O, tO
             lse[h, a:e] = ls[:, 0]
@@ -202,8 +203,8 @@ def attention_oracle(q, k, v, cu, scale, mask, dout):
             dk[keys, h // (H // G)] += scale * dS.t() @ Q
             tdk[keys, h // (H // G)] += scale * ((eds + n * dS.abs()).t() @ Q.abs())
             dv[keys, h // (H // G)] += P.t() @ dO
-            tdv[keys, h // (H // G)] += ((r + eP + n) * P).t() @ dO.abs()
-    tdq, tdk, tdv = (t * (1 + r) + r * x.abs() + 4 * U * x.abs() for t, x in ((tdq, dq), (tdk, dk), (tdv, dv)))
+            tdv[keys, h // (H // G)] += ((r + eP + n) * P + TINY).t() @ dO.abs()
+    tdq, tdk, tdv = (t * (1 + r) + r * x.abs() + 4 * U * x.abs() + TINY for t, x in ((tdq, dq), (tdk, dk), (tdv, dv)))
     return (o, lse, dq, dk, dv), (to, tl, tdq, tdk, tdv)
 
 
@@ -299,6 +300,85 @@ def test_attention_layouts():
     d = dout.new_ones(N, 1, 64)
     for a, b in zip(attention_all(far[:, :1], far[:, 1:2], far[:, 2:], cut, d), attention_all(near[:, :1], near[:, 1:2], near[:, 2:], cut, d)):
         assert torch.equal(a, b)
+
+
+def test_attention_more_than_2_31_elements():
+    """q, k, v, out and lse offsets past 32 bits of elements: 850 k tokens of 40 heads in 64-token sequences; the last ones
+    against the same tokens alone."""
+    N, H = 850_000 // 64 * 64, 40
+    assert N * H * 64 > 2 ** 31
+    g = gen(6)
+    one = randn(g, 64 * 50, 3 * H, 64).bfloat16()
+    qkv = one.repeat(-(-N // len(one)), 1, 1)[:N]
+    q, k, v = qkv[:, :H].contiguous(), qkv[:, H:2 * H], qkv[:, 2 * H:]
+    cu = torch.arange(N // 64 + 1, dtype=torch.int32, device="cuda") * 64
+    dout = q
+    got = attention_all(q, k, v, cu, dout)
+    small = attention_all(one[:, :H], one[:, H:2 * H], one[:, 2 * H:], cu[:51], one[:, :H])
+    m = (N // len(one)) * len(one)  # a whole copy ends here
+    for a, b in zip(got, small):
+        a = a[:, m - len(one):m] if a.dim() == 2 else a[m - len(one):m]
+        assert torch.equal(a, b)
+    del got, q, k, v, qkv, dout
+    torch.cuda.empty_cache()
+
+
+def test_attention_padded_batch_equals_packed():
+    """[B, L] with a key mask over the padding = the packed sequences, for the real tokens."""
+    lens, L = [70, 128, 1, 200], 200
+    q, k, v, cu, cut, dout, g = attention_inputs(41, lens, 4, 2, 64)
+    want = attention_all(q, k, v, cut, dout)
+    at = torch.cat([torch.arange(n) + i * L for i, n in enumerate(lens)]).cuda()
+    wide = lambda t: torch.randn(4 * L, *t.shape[1:], device="cuda", generator=g).bfloat16().index_copy(0, at, t.contiguous())
+    mask = torch.zeros(4 * L, dtype=torch.bool, device="cuda").index_fill(0, at, True)
+    d = wide(dout) * mask[:, None, None]
+    got = attention_all(wide(q), wide(k), wide(v), torch.arange(5, dtype=torch.int32, device="cuda") * L, d, mask=mask)
+    oracle, tol = attention_oracle(q, k, v, cu, 0.125, None, dout)
+    for a, b, t, n in zip(got, oracle, tol, ("out", "lse", "dq", "dk", "dv")):
+        within(a[:, at] if n == "lse" else a[at], b, t, n)
+    assert torch.equal(got[0][at], want[0]) and not got[3][~mask].any()
+
+
+def test_attention_rising_and_falling_scores():
+    """Keys whose scores rise from tile to tile by far more than the reference point may lag, and fall again; large values."""
+    N = 64 * 9
+    q = torch.zeros(N, 1, 64, device="cuda")
+    q[:, :, 0] = 8.0
+    g = gen(77)
+    k = 0.3 * randn(g, N, 1, 64)
+    k[:, 0, 0] = torch.tensor([0.0, 3, 8, 20, 45, 44, 10, -60, 45.5], device="cuda").repeat_interleave(64)
+    v = randn(g, N, 1, 64)
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    cut = torch.tensor([0, N], dtype=torch.int32, device="cuda")
+    dout = randn(g, N, 1, 64).bfloat16()
+    check_attention(q, k, v, [0, N], cut, dout)
+    check_attention(q, k.flip(0).contiguous(), (v * 1e30).bfloat16(), [0, N], cut, (dout * 1e-30).bfloat16())
+
+
+def test_empty_inputs():
+    e = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    cut = torch.zeros(3, dtype=torch.int32, device="cuda")
+    got = attention_all(e, e, e, cut, e)
+    assert got[0].shape == (0, 2, 64) and got[1].shape == (2, 0) and got[2].shape == got[3].shape == (0, 2, 64)
+    z, y = torch.empty(0, 7, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda")
+    for P in (1, 3):
+        ref = torch.randn(2 * P, device="cuda")
+        loss, logps, saved = T().preference_loss_forward(z, y, torch.zeros(2 * P + 1, dtype=torch.int32, device="cuda"), ref, beta=0.5)
+        want = torch.nn.functional.softplus(0.5 * (ref[0::2] - ref[1::2]).double()).mean().item()
+        assert abs(loss.item() - want) <= 1e-6 and not logps.any()
+        assert T().preference_loss_backward(z, y, saved).shape == (0, 7)
+
+
+def test_layer_norm_parameters_in_bf16_get_gradients_in_bf16():
+    g = gen(8)
+    x = randn(g, 40, 96).bfloat16().requires_grad_()
+    w, b = (1 + 0.1 * randn(g, 96)).bfloat16().requires_grad_(), randn(g, 96).bfloat16().requires_grad_()
+    dy = randn(g, 40, 96).bfloat16()
+    T().layer_norm(x, w, b).backward(dy)
+    want, tol = norm_oracle(x.detach(), w.detach(), b.detach(), dy)
+    for t, a, e in zip((x, w, b), want[1:], tol[1:]):
+        assert t.grad.dtype == torch.bfloat16
+        within(t.grad, a, e * (1 + R[torch.bfloat16]) + R[torch.bfloat16] * a.abs(), "bf16 parameters")
 
 
 def test_attention_offsets_outside_the_buffer_are_clamped():

@@ -49,7 +49,7 @@ def test_attention_entry_points_refuse():
     refused(fwd(H=0), INVALID, "heads=0")
     refused(fwd(N=-1), INVALID, "n_tokens=-1")
     refused(fwd(n=-1), INVALID, "n_segments=-1")
-    for s in (0.0, -1.0, float("nan"), float("inf")):
+    for s in (0.0, -1.0, 1e-31, float("nan"), float("inf")):
         refused(fwd(scale=s), INVALID, "scale")
     refused(fwd(cu=None), INVALID, "null")
     refused(fwd(q=None), INVALID, "null")
@@ -58,7 +58,8 @@ def test_attention_entry_points_refuse():
     refused(fwd(st=(128, 64, 128, 64, 128, 60, 128, 64)), INVALID, "tensor 2")
     refused(fwd(st=(128, 64, 128, 64, 128, 64, 56, 64)), INVALID, "tensor 3")
     refused(fwd(st=(1 << 23, 64, 128, 64, 128, 64, 128, 64)), INVALID, "tensor 0")
-    refused(fwd(N=2 ** 30, H=1024, G=1024), UNSUPPORTED, "grid")
+    refused(fwd(N=2 ** 30, H=1, G=1), UNSUPPORTED, "grid")
+    refused(fwd(N=2 ** 20, H=1024, G=1024), UNSUPPORTED, "grid")
     refused(fwd(N=2 ** 30 + 1), INVALID, "n_tokens")
     assert fwd(N=0, q=None) == 0
 
@@ -78,6 +79,7 @@ def test_preference_entry_points_refuse():
     refused(fwd(dt=5), INVALID, "dtype")
     refused(fwd(V=0), INVALID, "V=0")
     refused(fwd(N=-1), INVALID, "N=-1")
+    refused(fwd(N=1 << 26), UNSUPPORTED, "2^26")
     refused(fwd(n=0), INVALID, "n_pairs=0")
     refused(fwd(z=None), INVALID, "null")
     refused(fwd(cu=None), INVALID, "null")
@@ -85,7 +87,7 @@ def test_preference_entry_points_refuse():
     refused(fwd(saved=P + 8), INVALID, "16-byte")
     for e in (-0.1, 1.1, float("nan")):
         refused(fwd(e=e), INVALID, "label_smoothing")
-    refused(fwd(nb=4 * 16 + 8 - 1), WORKSPACE, "72 bytes")
+    refused(fwd(nb=4 * 16 + 16 - 1), WORKSPACE, "80 bytes")
     bwd = lambda z=P, dz=P, N=4: lib.esmk_pref_loss_bwd(z, L.F32, P, P, None, dz, N, 8, None)
     refused(bwd(dz=None), INVALID, "dlogits")
     refused(bwd(dz=P + 4), INVALID, "dlogits")
