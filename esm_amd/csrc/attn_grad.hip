@@ -17,6 +17,10 @@
 //
 // The backward pass is two kernels, each with one owner for every output element (no atomics, so the same inputs give the
 // same bits): dQ per query block (three products; it also forms delta), dK / dV per key block (four).
+//
+// Measured (forward, dQ, dK dV): 64 x 512 tokens, 18 heads of 64: 122, 172, 218 us - eight tiles per workgroup, so that a third
+// of its life is the load of the first rows and the store of the last; 4 x 4096, 40 heads of 64: 715, 988, 1284 us (960, 1040,
+// 1070 TFLOP/s) - matrix pipes 54 to 60 % busy at the clock the power limit leaves; a 2 TB/s share of HBM in both.
 #include <math.h>
 
 #include <type_traits>
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void a
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
     // p = exp2(c s - mc).  Any reference mc gives the same quotient, so it follows the row maximum only where it has to: it
     // is taken from the first tile with keys, and again when a tile's sum passes 2^16 (fp32 sums and bf16 probabilities have
-    // the range).  That spares the maximum over every tile.
+    // the range).  That spares the maximum over every tile (1136 -> 933 us at 4 x 4096 with the masks' own kernels).
     float mc = 0.f, l = 0.f;
     bool fresh = true;  // no reference yet
     for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
