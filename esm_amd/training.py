@@ -154,7 +154,7 @@ def _strided(t, what):
     tok, head, dim = t.stride()
     at = t.data_ptr()
     if dim != 1 or tok % 8 or head % 8 or at % 16 or not t.shape[2] <= tok < 2 ** 23:
-        t = t.contiguous()
+        t = t.clone(memory_format=_DENSE)  # contiguous() would keep an unaligned dense tensor, or one token's odd strides
         if t.shape[1] * t.shape[2] >= 2 ** 23:
             raise ValueError(f"{what}: a token of {t.shape[1]} heads x {t.shape[2]} is too wide")
         tok, head, dim = t.stride()

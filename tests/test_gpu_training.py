@@ -291,6 +291,20 @@ def test_attention_layouts():
             assert torch.equal(a, b)
     for a, b in zip(attention_all(q, k, v, cut, one), attention_all(q, k, v, cut, one.contiguous())):
         assert torch.equal(a, b)
+
+    def shifted(t):  # dense, at an address that is no multiple of 16 bytes
+        flat = t.new_empty(t.numel() + 1)[1:].view(t.shape)
+        return flat.copy_(t)
+    assert shifted(q).is_contiguous() and shifted(q).data_ptr() % 16
+    for a, b in zip(base, attention_all(shifted(q), shifted(k), shifted(v), cut, shifted(dout))):
+        assert torch.equal(a, b)
+    # one token and one head: torch calls any strides of theirs dense
+    lone = lambda t: t.new_empty(1, 1, 70)[:, :, :64].as_strided((1, 1, 64), (70, 3, 1)).copy_(t[:1, :1])
+    assert lone(q).is_contiguous()
+    first = cut.clamp(max=1)
+    for a, b in zip(attention_all(lone(q), lone(k), lone(v), first, lone(dout)),
+                    attention_all(q[:1, :1], k[:1, :1], v[:1, :1], first, dout[:1, :1])):
+        assert torch.equal(a, b)
     N = 400
     big = torch.empty(N * (2 ** 23 - 8), dtype=torch.bfloat16, device="cuda")
     far = big.as_strided((N, 3, 64), (2 ** 23 - 8, 64, 1))
