@@ -17,6 +17,7 @@
 namespace {
 
 constexpr int NG_MAX_D = 12288;      // 8 waves x 64 lanes x 24 elements
+constexpr int NG_MAX_M = 1 << 30;    // a row number plus the rows of a whole grid stays inside 31 bits
 constexpr int NG_FWD_GROUPS = 1024;  // four workgroups per CU; 512 to 2048 measure alike
 constexpr int NG_MAX_GROUPS = 512;   // of the backward pass, and so partial rows; 768 and 1024: 2 to 10 % slower
 
@@ -409,7 +410,7 @@ int norm_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const float* ga
 
 extern "C" int esmk_layernorm_fwd(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, void* y,
                                   float* stats, int M, int d, float eps, esmk_stream_t stream) {
-    if (M < 0 || d <= 0 || d > NG_MAX_D) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "esmk_layernorm_fwd: M=%d, d=%d (1..%d)", M, d, NG_MAX_D);
+    if (M < 0 || M > NG_MAX_M || d <= 0 || d > NG_MAX_D) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "esmk_layernorm_fwd: M=%d (0..2^30), d=%d (1..%d)", M, d, NG_MAX_D);
     if (dtype != ESMK_F32 && dtype != ESMK_BF16) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_fwd: bad dtype %d", dtype);
     if (M == 0) return ESMK_OK;
     if (!x || !gamma || !y || !stats) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_fwd: null pointer");
@@ -420,7 +421,7 @@ extern "C" int esmk_layernorm_fwd(const void* x, int dtype, int64_t ldx, const f
 }
 
 extern "C" size_t esmk_layernorm_bwd_workspace_bytes(int M, int d) {
-    if (M <= 0 || d <= 0 || d > NG_MAX_D) return 0;
+    if (M <= 0 || M > NG_MAX_M || d <= 0 || d > NG_MAX_D) return 0;
     const int G = ng_groups(M, d);
     return G == 1 ? 0 : (size_t)G * 2 * d * sizeof(float);
 }
@@ -428,7 +429,7 @@ extern "C" size_t esmk_layernorm_bwd_workspace_bytes(int M, int d) {
 extern "C" int esmk_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int dtype, const float* gamma,
                                   const float* stats, void* dx, float* dgamma, float* dbeta, void* workspace,
                                   size_t workspace_bytes, int M, int d, esmk_stream_t stream) {
-    if (M < 0 || d <= 0 || d > NG_MAX_D) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "esmk_layernorm_bwd: M=%d, d=%d (1..%d)", M, d, NG_MAX_D);
+    if (M < 0 || M > NG_MAX_M || d <= 0 || d > NG_MAX_D) ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "esmk_layernorm_bwd: M=%d (0..2^30), d=%d (1..%d)", M, d, NG_MAX_D);
     if (dtype != ESMK_F32 && dtype != ESMK_BF16) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_bwd: bad dtype %d", dtype);
     if (M == 0) {  // no rows: the parameters' gradients are zero
         if (dgamma || dbeta)

@@ -24,7 +24,6 @@ from . import _lib as L
 _DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 _F32, _BF16, _I32, _I64, _U8 = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.int64,), (torch.uint8,)
 _MASK = (torch.bool, torch.uint8)
-_INT_MAX = 2 ** 31 - 1
 _Strides8, _Strides16 = C.c_int64 * 8, C.c_int64 * 16
 Tensor, _DENSE = torch.Tensor, torch.contiguous_format
 
@@ -79,7 +78,7 @@ def _check_norm(x, weight, bias):
         if bias.shape != weight.shape:
             raise ValueError(f"bias {tuple(bias.shape)} does not fit x {tuple(shape)}")
     M = x.numel() // d
-    if M > _INT_MAX:
+    if M > 2 ** 30:
         raise ValueError("too many rows")
     return gpu, shape, M, d
 

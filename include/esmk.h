@@ -252,8 +252,8 @@ int esmk_attn_l64_d128(const void* qkv_bf16, void* ctx_bf16, const float* rope_c
  * ------------------------------------------------------------------------------------------ */
 
 /* y [M, d] = LayerNorm(x) and stats f32 [M][2] = (mean, 1/sqrt(var + eps)) of every row.  x, y: dtype (F32 or BF16);
- * x rows are ldx >= d elements apart, y rows d.  gamma f32 [d]; beta f32 [d] or NULL.  1 <= d <= 12288, any address that
- * suits the type.  stats 8-byte aligned. */
+ * x rows are ldx >= d elements apart, y rows d.  gamma f32 [d]; beta f32 [d] or NULL.  1 <= d <= 12288, M <= 2^30, any
+ * address that suits the type.  stats 8-byte aligned. */
 int esmk_layernorm_fwd(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, void* y, float* stats,
                        int M, int d, float eps, esmk_stream_t stream);
 /* dx [M, d] (dtype, dense rows); dgamma, dbeta f32 [d], overwritten (either may be NULL: not wanted).  dy, x: dtype, rows

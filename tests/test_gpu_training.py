@@ -673,6 +673,7 @@ def test_refusals_name_the_argument():
             (ValueError, lambda: t.layer_norm_backward(x, x, w, st[:2])),
             (ValueError, lambda: t.layer_norm_forward(torch.zeros(1, 12289, device="cuda"), torch.ones(12289, device="cuda"))),
             (TypeError, lambda: t.attention_varlen_forward(q.float(), q, q, cu)),
+            (ValueError, lambda: t.layer_norm_forward(x[:1, :1].expand(2 ** 30 + 1, 1), w[:1])),
             (ValueError, lambda: t.attention_varlen_forward(q[:, :, :32], q[:, :, :32], q[:, :, :32], cu)),
             (ValueError, lambda: t.attention_varlen_forward(q, q[:, :1].expand(8, 3, 64), q[:, :1].expand(8, 3, 64), cu)),
             (ValueError, lambda: t.attention_varlen_forward(q, q[:4], q[:4], cu)),

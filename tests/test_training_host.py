@@ -23,6 +23,7 @@ def test_layernorm_entry_points_refuse():
     refused(fwd(d=0), UNSUPPORTED, "d=0")
     refused(fwd(d=12289, ld=12289), UNSUPPORTED, "12289")
     refused(fwd(M=-1), UNSUPPORTED, "M=-1")
+    refused(fwd(M=2 ** 31 - 1, d=1), UNSUPPORTED, "M=2147483647")  # a row number plus the grid's rows would pass 31 bits
     refused(fwd(dt=2), INVALID, "dtype")
     refused(fwd(ld=63), INVALID, "row stride")
     refused(fwd(st=P + 4), INVALID, "stats")
@@ -34,6 +35,7 @@ def test_layernorm_entry_points_refuse():
     refused(bwd(dy=None), INVALID, "null")
     refused(bwd(ldg=1), INVALID, "row stride")
     refused(bwd(dt=7), INVALID, "dtype")
+    refused(bwd(M=2 ** 30 + 1), UNSUPPORTED, "M=1073741825")
     refused(bwd(ws=None), WORKSPACE, "workspace")
     refused(bwd(nb=lib.esmk_layernorm_bwd_workspace_bytes(4096, 64) - 1), WORKSPACE, "workspace")
     assert lib.esmk_layernorm_bwd_workspace_bytes(0, 64) == 0 and lib.esmk_layernorm_bwd_workspace_bytes(4096, 64) > 0
