@@ -328,7 +328,8 @@ extern "C" int esmk_pref_loss_fwd(const void* logits, int dtype, const int64_t* 
                                   int N, int V, void* saved, size_t saved_bytes, float* logps, float* loss,
                                   esmk_stream_t stream) {
     if (int rc = pl_check("esmk_pref_loss_fwd", logits, dtype, targets, saved, N, V)) return rc;
-    if (n_pairs <= 0 || n_pairs > (1 << 29)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: n_pairs=%d", n_pairs);
+    if (n_pairs <= 0 || n_pairs >= (1 << 23))  // a launch holds fewer than 2^32 threads, PL_PAIR a pair
+        ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: n_pairs=%d (1..2^23 - 1)", n_pairs);
     if (!cu_seqlens || !ref_logps || !logps || !loss || !saved) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: null pointer");
     if (!(label_smoothing >= 0.0 && label_smoothing <= 1.0)) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_pref_loss_fwd: label_smoothing outside [0, 1]");
     if (saved_bytes < esmk_pref_loss_saved_bytes(N, n_pairs))

@@ -296,6 +296,8 @@ def preference_loss_forward(logits, targets, cu_seqlens, ref_logps, beta: float 
     P = (cu_seqlens.numel() - 1) // 2
     if cu_seqlens.dim() != 1 or P < 1 or cu_seqlens.numel() != 2 * P + 1 or not cu_seqlens.is_contiguous():
         raise ValueError("cu_seqlens must be a dense vector of 2 * pairs + 1 offsets, one pair at least")
+    if P >= 2 ** 23:
+        raise ValueError("too many pairs")
     if ref_logps.shape != (2 * P,):
         raise ValueError(f"ref_logps {tuple(ref_logps.shape)}: wanted ({2 * P},)")
     if not 0.0 <= label_smoothing <= 1.0:

@@ -285,7 +285,7 @@ int esmk_attn_varlen_bwd(const void* dout, const void* q, const void* k, const v
                          const uint8_t* key_mask, int n_tokens, int n_heads, int n_kv_heads, int head_dim, float scale,
                          void* workspace, size_t workspace_bytes, esmk_stream_t stream);
 
-/* Preference loss over n_pairs >= 1 pairs of packed sequences: sequence 2i is the preferred one of pair i, 2i + 1 the other.
+/* Preference loss over n_pairs (1 .. 2^23 - 1) pairs of packed sequences: sequence 2i is the preferred one of pair i, 2i + 1 the other.
  *   logps[s] = sum of log softmax(logits[t])[targets[t]] over the scored tokens of sequence s
  *   m_i      = beta ((logps[2i] - ref_logps[2i]) - (logps[2i+1] - ref_logps[2i+1]))
  *   loss     = mean_i [(1 - e) softplus(-m_i) + e softplus(m_i) - nll_weight logps[2i] / max(1, scored tokens of 2i)]

@@ -685,6 +685,7 @@ def test_refusals_name_the_argument():
             (ValueError, lambda: t.preference_loss_forward(z, y[:4], cp, ref)),
             (ValueError, lambda: t.preference_loss_forward(z, y, cu, ref)),
             (ValueError, lambda: t.preference_loss_forward(z, y, cp, ref[:1])),
+            (ValueError, lambda: t.preference_loss_forward(z, y, cp[:1].expand(2 ** 24 + 1).contiguous(), ref)),
             (ValueError, lambda: t.preference_loss_forward(z, y, cp, ref, label_smoothing=1.5)),
             (TypeError, lambda: t.preference_loss_forward(z, y.int(), cp, ref)),
             (ValueError, lambda: t.preference_loss_backward(z, y, torch.zeros(8, device="cuda")))):

@@ -83,6 +83,7 @@ def test_preference_entry_points_refuse():
     refused(fwd(N=-1), INVALID, "N=-1")
     refused(fwd(N=1 << 26), UNSUPPORTED, "2^26")
     refused(fwd(n=0), INVALID, "n_pairs=0")
+    refused(fwd(n=1 << 23, nb=1 << 40), INVALID, "n_pairs=8388608")  # 512 threads a pair: 2^32
     refused(fwd(z=None), INVALID, "null")
     refused(fwd(cu=None), INVALID, "null")
     refused(fwd(z=P + 4), INVALID, "16-byte")
