@@ -132,6 +132,28 @@ def test_layer_norm_far_rows():
         assert torch.equal(a, b)
 
 
+def test_layer_norm_more_than_2_31_elements():
+    """Dense rows past 2^32 bytes of x, y, dy and dx: the last rows against the same rows alone, and column sums of rows that
+    repeat."""
+    g = gen(4)
+    one, dy1 = randn(g, 1024, 1152).bfloat16(), randn(g, 1024, 1152).bfloat16()
+    w, b = 1 + 0.1 * randn(g, 1152), 0.1 * randn(g, 1152)
+    times = 1850
+    x, dy = one.repeat(times, 1), dy1.repeat(times, 1)
+    assert x.numel() > 2 ** 31
+    y, st = T().layer_norm_forward(x, w, b)
+    dx, dw, db = T().layer_norm_backward(dy, x, w, st)
+    y1, st1 = T().layer_norm_forward(one, w, b)
+    dx1, _, _ = T().layer_norm_backward(dy1, one, w, st1)
+    for got, want in ((y, y1), (st, st1), (dx, dx1)):
+        assert torch.equal(got[-1024:], want) and torch.equal(got[:1024], want)
+    want, tol = norm_oracle(one, w, b, dy1)
+    # a lane adds 1850 x 1024 / 512 rows of its workgroup's four slots, then 64 more sums: below 1000 u of the magnitudes
+    h = ((one.double() - one.double().mean(-1, keepdim=True)) / (one.double().var(-1, unbiased=False, keepdim=True) + 1e-5).sqrt())
+    within(dw, times * want[2], times * (tol[2] + 1000 * U * (dy1.double() * h).abs().sum(0)), "dw")
+    within(db, times * want[3], times * (tol[3] + 1000 * U * dy1.double().abs().sum(0)), "db")
+
+
 def test_layer_norm_autograd_and_differences():
     g = gen(11)
     x, w, b = randn(g, 21, 130), 1 + 0.2 * randn(g, 130), 0.2 * randn(g, 130)
@@ -461,9 +483,9 @@ def preference_oracle(z, y, cu, ref, beta, eps, alpha, dtype):
     return (loss, torch.stack(l), dz), (tloss + 4 * U * abs(loss), torch.stack(tl) + U * torch.stack(l).abs(), tdz)
 
 
-def preference_inputs(seed, lens, V, dtype, tail=0, spread=1.5):
+def preference_inputs(seed, lens, V, dtype, tail=0, spread=1.5, lead=0):
     g = gen(seed)
-    cu = [0]
+    cu = [lead]
     for n in lens:
         cu.append(cu[-1] + n)
     N = cu[-1] + tail
@@ -489,6 +511,33 @@ def test_preference_loss(V, lens, tail, dtype):
         for got, a, t, n in zip((loss, logps, dz), want, tol, ("loss", "logps", "dz")):
             within(got, a, t, n)
         assert dz.dtype == dtype and not dz[(y < 0) | (y >= V)].any() and not dz[cu[-1]:].any()
+
+
+@pytest.mark.parametrize("lens", [[2500, 700, 1, 5000], [513, 2049, 512, 2048], [3] * 1300])
+def test_preference_long_sequences_many_pairs_and_a_lead(lens):
+    """Sequences beyond one turn of a workgroup, more pairs than a workgroup has threads, tokens before the first sequence."""
+    z, y, cu, cut, ref, _ = preference_inputs(len(lens), lens, 33, torch.float32, tail=3, lead=11)
+    loss, logps, saved = T().preference_loss_forward(z, y, cut, ref, 0.02, 0.1, 0.3)
+    dz = T().preference_loss_backward(z, y, saved)
+    want, tol = preference_oracle(z, y, cu, ref, 0.02, 0.1, 0.3, torch.float32)
+    for got, a, t, n in zip((loss, logps, dz), want, tol, ("loss", "logps", "dz")):
+        within(got, a, t, n)
+    assert not dz[:11].any() and not dz[cu[-1]:].any()
+
+
+def test_preference_more_than_2_31_elements():
+    """Logits and gradients past 2^32 bytes: the last pair against the same pair alone (half the weight among two pairs)."""
+    z1, y1, cu, cut, ref, _ = preference_inputs(19, [300, 211], 4096, torch.bfloat16)
+    times = 1040
+    z, y = z1.repeat(times, 1), y1.repeat(times)
+    assert z.numel() > 2 ** 31
+    N = len(y)
+    cu2 = torch.tensor([0, 400, N - 511, N - 211, N], dtype=torch.int32, device="cuda")
+    loss, logps, saved = T().preference_loss_forward(z, y, cu2, torch.cat([ref, ref]))
+    dz = T().preference_loss_backward(z, y, saved)
+    a, b, c = T().preference_loss_forward(z1, y1, cut, ref)
+    assert torch.equal(logps[2:], b)
+    assert torch.equal(dz[-511:], T().preference_loss_backward(z1, y1, c, torch.full((), 0.5, device="cuda")))
 
 
 def test_preference_skipped_tokens_may_hold_anything():
