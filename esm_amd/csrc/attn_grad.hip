@@ -9,8 +9,8 @@
 //
 // Matrix products run on v_mfma_f32_32x32x16_bf16 with fp32 accumulators.  A product's operand that lives in the lanes is
 // held in registers for the whole kernel (queries in the forward and dQ kernels, keys in the dK / dV kernel); the other
-// side streams through a two-slot LDS ring of 64-row tiles, filled by LDS-DMA one tile ahead.  Scores are formed with the
-// resident side on the lanes and the streamed side in the registers, so the exponentiated tile converts in place (bf16,
+// side streams through a two-slot LDS ring of 64- or 32-row tiles, filled by LDS-DMA one tile ahead.  Scores are formed with
+// the resident side on the lanes and the streamed side in the registers, so the exponentiated tile converts in place (bf16,
 // the second operand of the MFMA that consumes it) and softmax statistics stay in fp32.  The transposed operand of the
 // second product is read from the same row-major tile with ds_read_b64_tr_b16: the LDS image's 16-byte chunks are
 // XOR-swizzled by a function of the row that keeps both the row reads and the transposed reads free of bank conflicts.
@@ -29,7 +29,7 @@
 
 namespace {
 
-constexpr int TR = 64;       // rows of a streamed tile
+constexpr int TR = 64;       // rows of a streamed tile, where a kernel does not say 32
 constexpr int AG_WAVES = 4;
 constexpr float AG_LOG2E = 1.4426950408889634f, AG_LN2 = 0.6931471805599453f;
 
@@ -45,7 +45,7 @@ struct OutView {
     int64_t tok, head;
 };
 
-// ---- LDS image of a 64-row tile: row r at r * 2D bytes, its 16-byte chunk c at c ^ swz(r) -----------------------------
+// ---- LDS image of a tile: row r at r * 2D bytes, its 16-byte chunk c at c ^ swz(r) -----------------------------
 //   row reads (32 rows, one logical chunk, ds_read_b128): 16 consecutive rows cover all 64 banks
 //   transposed reads (rows 4h..4h+3, 64 bytes each, ds_read_b64_tr_b16): the four rows cover all 64 banks
 template <int D>
@@ -283,11 +283,11 @@ __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict
     return first < s.len;
 }
 
-// Which keys of a 64-key tile take part, one bit each; `row` is this lane's key.
+// Which keys of a tile take part, one bit each; `row` is this lane's key.
 __device__ __forceinline__ unsigned char mask_byte(const unsigned char* mask, int64_t s0, int row, int len) {
     return row < len ? (mask ? mask[s0 + row] : 1) : 0;
 }
-// Accumulator start of 32 scores from a row of 64 floats in LDS (0, or -inf where the key takes no part): masking costs
+// Accumulator start of 32 scores from a tile's row of floats in LDS (0, or -inf where the key takes no part): masking costs
 // the row reads and no vector instruction.
 __device__ __forceinline__ f32x16 rows16(const float* st, int mt, int hi) {
     f32x16 r;
@@ -306,46 +306,47 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
 // The key side of the forward and dQ kernels: K and V tiles through the ring, key masks, and the loop over the tiles.
 // MASK instantiations take every tile through the biased path; the others only a last tile that is not full, behind the
 // loop (one path inside the loop: a second one costs a copy of the accumulators per tile).
-template <int D, bool MASK, typename F>
+template <int D, int KT, bool MASK, typename F>
 __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, const unsigned char* mask, const Span& sp, int kvh,
-                                              char* smem, float (*bias)[TR], int wave, int lane, F tile) {
-    constexpr int TILE = TR * 2 * D, SLOT = 2 * TILE;
+                                              char* smem, float (*bias)[KT], int wave, int lane, F tile) {
+    constexpr int TILE = KT * 2 * D, SLOT = 2 * TILE;
     const __bf16* kb = k.p + sp.s0 * k.tok + kvh * k.head;
     const __bf16* vb = v.p + sp.s0 * v.tok + kvh * v.head;
-    Stage<D> sk, sv;
+    Stage<D, KT> sk, sv;
     sk.init(k.tok, wave, lane);
     sv.init(v.tok, wave, lane);
-    const int nt = (sp.len + TR - 1) / TR;
+    const int nt = (sp.len + KT - 1) / KT;
+    auto mask_at = [&](int t) -> unsigned char { return KT == 64 || lane < KT ? mask_byte(mask, sp.s0, t * KT + lane, sp.len) : 0; };
     auto stage = [&](int slot, int kt, unsigned long long bits) {
         char* base = smem + slot;
-        const __bf16 *kp = kb + (int64_t)kt * TR * k.tok, *vp = vb + (int64_t)kt * TR * v.tok;
+        const __bf16 *kp = kb + (int64_t)kt * KT * k.tok, *vp = vb + (int64_t)kt * KT * v.tok;
         if constexpr (MASK) {
-            sk.go_masked(base, kp, sp.len - kt * TR, wave, lane, bits);
-            sv.go_masked(base + TILE, vp, sp.len - kt * TR, wave, lane, bits);
+            sk.go_masked(base, kp, sp.len - kt * KT, wave, lane, bits);
+            sv.go_masked(base + TILE, vp, sp.len - kt * KT, wave, lane, bits);
         } else {
-            sk.go(base, kp, sp.len - kt * TR, wave);
-            sv.go(base + TILE, vp, sp.len - kt * TR, wave);
+            sk.go(base, kp, sp.len - kt * KT, wave);
+            sv.go(base + TILE, vp, sp.len - kt * KT, wave);
         }
     };
     unsigned long long bits = 0;  // of tile kt
     unsigned char mb = 0;         // of tile kt + 1
     if constexpr (MASK) {
-        bits = __ballot(mask_byte(mask, sp.s0, lane, sp.len) != 0);
-        mb = mask_byte(mask, sp.s0, TR + lane, sp.len);
+        bits = __ballot(mask_at(0) != 0);
+        mb = mask_at(1);
     }
     stage(0, 0, bits);
-    const int nloop = MASK ? nt : sp.len / TR;
+    const int nloop = MASK ? nt : sp.len / KT;
     for (int kt = 0; kt < nloop; ++kt) {
         const int cur = (kt & 1) * SLOT;
         if constexpr (MASK)
-            if (wave == 0) bias[kt & 1][lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
+            if (wave == 0 && (KT == 64 || lane < KT)) bias[kt & 1][lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();  // tile kt has landed for every wave, and the other slot is read by none
         __builtin_amdgcn_sched_barrier(0);
         const unsigned long long now = bits;
         if constexpr (MASK) {
             bits = __ballot(mb != 0);
-            mb = mask_byte(mask, sp.s0, (kt + 2) * TR + lane, sp.len);
+            mb = mask_at(kt + 2);
         }
         if (kt + 1 < nt) stage(SLOT - cur, kt + 1, bits);
         if constexpr (MASK)
@@ -354,7 +355,7 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
     }
     if (!MASK && nloop < nt) {  // rows past the end landed as zeros
         const int cur = (nloop & 1) * SLOT;
-        if (wave == 0) bias[0][lane] = nloop * TR + lane < sp.len ? 0.f : -INFINITY;
+        if (wave == 0 && (KT == 64 || lane < KT)) bias[0][lane] = nloop * KT + lane < sp.len ? 0.f : -INFINITY;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
@@ -363,14 +364,16 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
+// Key tiles of 64 rows at head dim 64 (32: 10 % slower, twice the barriers), of 32 at 128: half the score registers and LDS
+// make room for a third wave per SIMD (64 x 512, 9 heads of 128: 124 -> 109 us; 24 ragged, 16 heads, masked: 172 -> 163 us).
 template <int D, bool MASK>
-__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 3) void attn_fwd_lse_kernel(View q, View k, View v, OutView o,
                                                                      float* __restrict__ lse, const int* __restrict__ cu,
                                                                      int n_seg, const unsigned char* __restrict__ mask,
                                                                      int N, int group, Order od, float c) {
-    constexpr int TILE = TR * 2 * D;
+    constexpr int KT = D == 64 ? 64 : 32, MT = KT / 32, TILE = KT * 2 * D;
     __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
-    __shared__ __attribute__((aligned(16))) float bias[2][TR];
+    __shared__ __attribute__((aligned(16))) float bias[2][KT];
     const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int head;
@@ -410,17 +413,17 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void a
     // the range).  That spares the maximum over every tile (1136 -> 933 us at 4 x 4096 with the masks' own kernels).
     float mc = 0.f, l = 0.f;
     bool fresh = true;  // no reference yet
-    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
+    for_key_tiles<D, KT, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
-        f32x16 s[2];
+        f32x16 s[MT];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) s[mt] = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
-        bf16x8 p[2][2];
+        for (int mt = 0; mt < MT; ++mt) s[mt] = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
+        bf16x8 p[MT][2];
         float ps;
         auto probabilities = [&] {
             ps = 0.f;
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < MT; ++mt) {
                 float e[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -435,9 +438,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void a
         auto largest = [&] {
             float mx = s[0][0];
 #pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[0][r]);
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[1][r]);
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
             mx = half_max(mx) * c;
             return mx == -INFINITY ? 0.f : mx;
         };
@@ -459,7 +462,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 2) void a
         }
         l += ps;
         mfma_tr<D, 0>(acc, ta, lds0 + cur + TILE, p[0]);
-        mfma_tr<D, 1>(acc, ta, lds0 + cur + TILE, p[1]);
+        if constexpr (MT == 2) mfma_tr<D, 1>(acc, ta, lds0 + cur + TILE, p[1]);
     });
     l = half_sum(l);
     // no key: zeros; NaN stays
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
     const f32x16 nd = splat16(-dl);  // dP starts from -delta
 
-    for_key_tiles<D, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
+    for_key_tiles<D, TR, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
         auto half = [&](auto mt_) {
             constexpr int mt = decltype(mt_)::value;
