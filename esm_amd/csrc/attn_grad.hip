@@ -305,8 +305,9 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
 
 // The key side of the forward and dQ kernels: K and V tiles through the ring, key masks, and the loop over the tiles.
 // MASK instantiations take every tile through the biased path; the others only a last tile that is not full, behind the
-// loop (one path inside the loop: a second one costs a copy of the accumulators per tile).
-template <int D, int KT, bool MASK, typename F>
+// loop (one path inside the loop: a second one costs a copy of the accumulators per tile).  LONE: the only tile of a
+// sequence goes there too, and `tile` is told.
+template <int D, int KT, bool MASK, bool LONE, typename F>
 __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, const unsigned char* mask, const Span& sp, int kvh,
                                               char* smem, float (*bias)[KT], int wave, int lane, F tile) {
     constexpr int TILE = KT * 2 * D, SLOT = 2 * TILE;
@@ -335,7 +336,7 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
         mb = mask_at(1);
     }
     stage(0, 0, bits);
-    const int nloop = MASK ? nt : sp.len / KT;
+    const int nloop = LONE && nt == 1 ? 0 : MASK ? nt : sp.len / KT;
     for (int kt = 0; kt < nloop; ++kt) {
         const int cur = (kt & 1) * SLOT;
         if constexpr (MASK)
@@ -351,15 +352,16 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
         if (kt + 1 < nt) stage(SLOT - cur, kt + 1, bits);
         if constexpr (MASK)
             if (now == 0) continue;  // every wave has the same bits
-        tile(std::integral_constant<bool, MASK>{}, cur, bias[kt & 1]);
+        tile(std::integral_constant<bool, MASK>{}, false, cur, bias[kt & 1]);
     }
-    if (!MASK && nloop < nt) {  // rows past the end landed as zeros
+    if ((LONE || !MASK) && nloop < nt) {  // rows past the end landed as zeros
         const int cur = (nloop & 1) * SLOT;
-        if (wave == 0 && (KT == 64 || lane < KT)) bias[0][lane] = nloop * KT + lane < sp.len ? 0.f : -INFINITY;
+        const bool in = MASK ? (bits >> lane) & 1 : nloop * KT + lane < sp.len;
+        if (wave == 0 && (KT == 64 || lane < KT)) bias[0][lane] = in ? 0.f : -INFINITY;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        tile(std::true_type{}, cur, bias[0]);
+        if (!MASK || bits != 0) tile(std::true_type{}, LONE && nt == 1, cur, bias[0]);
     }
 }
 
@@ -413,7 +415,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 3) void a
     // the range).  That spares the maximum over every tile (1136 -> 933 us at 4 x 4096 with the masks' own kernels).
     float mc = 0.f, l = 0.f;
     bool fresh = true;  // no reference yet
-    for_key_tiles<D, KT, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
+    for_key_tiles<D, KT, MASK, false>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, bool, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
         f32x16 s[MT];
 #pragma unroll
@@ -514,15 +516,28 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
     dl = half_sum(dl);
     const float c = scale * AG_LOG2E;
     const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;  // +inf only where every tile is skipped
-    if (on && hi == 0) delta[(int64_t)head * N + tok] = dl;
     const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
-    const f32x16 nd = splat16(-dl);  // dP starts from -delta
+    f32x16 nd = splat16(-dl);  // dP starts from -delta
 
-    for_key_tiles<D, TR, MASK>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
+    for_key_tiles<D, TR, MASK, true>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, bool lone, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
+        // delta + rowsum(P (dP - delta)) is delta without the rounding of out, which counts where few keys are averaged: dq of
+        // 20 .. 64 tokens is off by 2.4e-3 instead of 2.6e-3 (2.4e-3 is the rounding of dS and dq), of one token by nothing.
+        // For a sequence of one tile it costs two products more and no reads (500 x 64 tokens, backward pass: 232 -> 236 us).
+        if (BIASED && lone) {
+            float more = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, rows16(st, mt, hi));
+                const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], gf, nd);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) more += __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
+            }
+            nd = splat16(nd[0] - half_sum(more));
+        }
         auto half = [&](auto mt_) {
             constexpr int mt = decltype(mt_)::value;
             const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
@@ -536,6 +551,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
         half(std::integral_constant<int, 0>{});
         half(std::integral_constant<int, 1>{});
     });
+    if (on && hi == 0) delta[(int64_t)head * N + tok] = -nd[0];
     store_row<D>(op, acc, scale, hi, on);
 }
 

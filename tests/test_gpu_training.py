@@ -180,11 +180,12 @@ def test_layer_norm_autograd_and_differences():
 
 # ------------------------------------------------------------------------------------------------ attention
 
-def attention_oracle(q, k, v, cu, scale, mask, dout):
+def attention_oracle(q, k, v, cu, scale, mask, dout, short=False):
     """64-bit (out, lse, dq, dk, dv) and bounds.  Where the kernels round: P to bf16 before P V and P^T dO (r), dS to bf16
     before dS K and dS^T Q (r), outputs (r); delta uses the rounded out.  fp32: a score has D products (D u of their
     magnitudes) and moves P by that, relatively; sums over keys or queries L u.  Below the smallest normal number, 2^-126, a
-    probability or a result may be flushed to zero: that much is added wherever one enters."""
+    probability or a result may be flushed to zero: that much is added wherever one enters.  short: sequences of at most 64
+    tokens, where delta is summed again as delta + rowsum(P (dP - delta)) and out's rounding leaves it."""
     r = R[torch.bfloat16]
     N, H, D = q.shape
     G = k.shape[1]
@@ -215,6 +216,9 @@ def attention_oracle(q, k, v, cu, scale, mask, dout):
             dS = P * (dP - dl)
             eDl = (dO.abs() * tO).sum(-1, keepdim=True) + (D + 8) * U * (dO * O).abs().sum(-1, keepdim=True)
             eDP = (D + 8) * U * (dO.abs() @ V.abs().t())
+            if short:
+                assert L <= 64
+                eDl = ((eP + (L + 32) * U) * P * ((dP - dl).abs() + eDl) + P * eDP).sum(-1, keepdim=True) + 2 * U * dl.abs()
             eds = P * (eDl + eDP + eP * (dP - dl).abs()) * (1 + r) + r * dS.abs() + TINY * (1 + (dP - dl).abs())  # abs, of the rounded dS
             n = (L + 32) * U
             o[a:e, h], to[a:e, h] = O, tO
@@ -266,6 +270,22 @@ def check_attention(q, k, v, cu, cut, dout, scale=None, mask=None):
 def test_attention(lens, H, G, tail, D):
     q, k, v, cu, cut, dout, _ = attention_inputs(len(lens) * 7 + D, lens, H, G, D, tail)
     check_attention(q, k, v, cu, cut, dout)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_short_sequences_have_an_exact_delta(D, masked):
+    """dq and dk of sequences of one tile: what the rounding of out would leave in delta (all of dq and dk, for one token,
+    where they are zero) is above these bounds."""
+    q, k, v, cu, cut, dout, g = attention_inputs(50 + D, [1, 5, 64, 2, 33, 1, 63, 3] * 3, 4, 2, D, tail=2)
+    mask = None
+    if masked:
+        mask = torch.rand(len(q), generator=g, device="cuda") > 0.2
+        mask[cu[2]:cu[3]] = False
+    got = attention_all(q, k, v, cut, dout, mask=mask)
+    want, tol = attention_oracle(q, k, v, cu, D ** -0.5, mask, dout, short=True)
+    for a, b, t, n in zip(got[2:], want[2:], tol[2:], ("dq", "dk", "dv")):
+        within(a, b, t, n)
 
 
 @pytest.mark.parametrize("D", [64, 128])
