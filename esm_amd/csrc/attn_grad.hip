@@ -217,16 +217,18 @@ __device__ __forceinline__ void store_row(__bf16* row, const f32x16 (&o)[D / 32]
 // N / 128 + n + 2 is known without reading cu_seqlens, and a block finds its stretch by search.  Offsets are clamped into
 // [0, N]: a bad cu_seqlens cannot lead outside the buffers.
 //
-// Order of the blocks: the blocks of a head over about one sequence are a group, and groups (all heads of a sequence, then
-// the next) are dealt to the eight XCDs in turn.  A group shares its keys in one XCD's L2, the XCDs together read whole rows
-// of a fused qkv buffer, and sequences of unequal length load all XCDs alike.  Within an XCD four groups advance together:
-// its workgroups go to its shader engines in turn, and a group's block numbers without rows would otherwise fall to the same
-// engines every time (128-token sequences: every second number; forward pass 118 -> 86 us).
+// Order of the blocks above 62 sequences (find_span_even() for fewer): the blocks of a head over about one sequence are a
+// group, and groups (all heads of a sequence, then the next) are dealt to the eight XCDs in turn.  A group shares its keys in one
+// XCD's L2, the XCDs together read whole rows of a fused qkv buffer, and sequences of unequal length load all XCDs alike.  Within
+// an XCD four groups advance together: its workgroups go to its shader engines in turn, and a group's block numbers without rows
+// would otherwise fall to the same engines every time (128-token sequences: every second number; forward pass 118 -> 86 us).
 constexpr int AG_BLK = 128;  // rows a workgroup owns
 struct Order {
     int n_blk, chunk, heads, grid;       // chunk: block numbers of an average sequence
     unsigned by_chunk, by_heads;         // reciprocals, see quotient()
     float per_blk;                       // stretches per block number
+    bool even, by_length;                // find_span_even()
+    unsigned by_eights, by_rest;         // reciprocals of heads & ~7 and heads & 7
 };
 struct Span {
     int64_t s0;
@@ -238,9 +240,65 @@ __device__ __forceinline__ int quotient(int n, int d, unsigned m) {
     const int q = (int)__umulhi((unsigned)n, m);
     return n - q * d >= d ? q + 1 : q;
 }
+// Up to 62 sequences, one lane per stretch: block numbers without gaps, dealt to the XCDs one by one, where groups load them
+// unequally as soon as there are few.  Measured by groups and so: one sequence of 8192, 10 heads of 64: forward pass 414 and 217
+// us, backward 1310 and 622; 24 of 217 to 1031, 16 : 4 heads of 128, backward 541 and 436; 60 of 512, 18 heads of 64: 107, 345 and
+// 106, 344; 10 of 2048, 16 heads of 128: 355, 1166 and 378, 1228, the most it loses.  Above 62 sequences counting costs short ones
+// more than gaps do (250 of 20 to 130, backward: 140 and 147).
+// In a stretch the heads go round the XCDs in eights, so that the blocks of a head share its keys in one L2 (all heads at a
+// time: 60 of 512, 9 heads: 59 and 69 us), and what is left of the heads block by block.  Long sequences come in the order of
+// their lengths, so that the last workgroups to start are the shortest (24 of 217 to 1031 above: nearly half of what is gained;
+// below 512 tokens on average it costs more than it gives): a lane adds up the blocks of the stretches that come before its own.
+constexpr int EVEN_MAX = 64, EVEN_LONG = 512;
+__device__ __forceinline__ int scan64(int v) {  // sum over this lane and those before it
+    auto add = [&](auto ctrl, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // from the lane 1, 2, 4, 8 before, in 16
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // from the 16, then the 32, before
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+    return v;
+}
+__device__ __forceinline__ bool find_span_even(const Order& od, const int* __restrict__ cu, int n, int N, int& head, Span& s) {
+    const int lane = threadIdx.x & 63, b = blockIdx.x;
+    auto start = [&](int i) { return i <= 0 ? 0 : i >= n + 2 ? N : min(max(cu[i - 1], 0), N); };
+    auto lane_of = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
+    const int from = start(lane), len = max(start(lane + 1) - from, 0), blocks = (len + AG_BLK - 1) / AG_BLK;
+    const bool live = lane >= 1 && lane <= n;
+    int before = 0;
+    if (!od.by_length || __ballot(live && len != lane_of(len, 1)) == 0) {  // all alike: nothing to order
+        before = scan64(blocks) - blocks;
+    } else {
+        const int key = (live ? blocks : 0) * 64 + 63 - lane;
+        for (int j0 = 0; j0 < n + 2; j0 += 8)
+#pragma unroll
+            for (int j = j0; j < j0 + 8; ++j)  // lanes past the last stretch have no blocks
+                before += lane_of(key, j) > key ? lane_of(blocks, j) : 0;
+    }
+    before *= od.heads;
+    const unsigned long long mine = __ballot(b >= before && b < before + blocks * od.heads);
+    if (mine == 0) return false;
+    const int o = (int)__builtin_ctzll(mine), eights = od.heads & ~7, of_eights = lane_of(blocks, o) * eights;
+    int r = b - lane_of(before, o), blk;
+    if (r < of_eights) {
+        blk = quotient(r, eights, od.by_eights);
+        head = r - blk * eights;
+    } else {
+        r -= of_eights;
+        blk = quotient(r, od.heads & 7, od.by_rest);
+        head = eights + r - blk * (od.heads & 7);
+    }
+    s.s0 = lane_of(from, o);
+    s.len = lane_of(len, o);
+    s.first = blk * AG_BLK;
+    s.dead = o == 0 || o == n + 1;
+    return true;
+}
 // false: no such block (uniform over the workgroup).  Everything here is on the scalar side, and for sequences of about
 // equal length one read of eight offsets settles it (a vector search took 4500 cycles of a 512-token block's 40000).
 __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict__ cu, int n, int N, int& head, Span& s) {
+    if (od.even) return find_span_even(od, cu, n, N, head, s);
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;  // blocks go to the XCDs round-robin
     const int four = at >> 2, turn = quotient(four, od.chunk, od.by_chunk), group = (turn * 4 + (at & 3)) * 8 + xcd;
     const int c = quotient(group, od.heads, od.by_heads);
@@ -700,6 +758,11 @@ Order ag_order(int N, int n_seg, int heads) {
     o.by_chunk = 0xffffffffu / (unsigned)o.chunk;
     o.by_heads = 0xffffffffu / (unsigned)heads;
     o.per_blk = (float)(n_seg + 2) / (float)o.n_blk;
+    o.by_eights = heads >= 8 ? 0xffffffffu / (unsigned)(heads & ~7) : 0u;
+    o.by_rest = heads & 7 ? 0xffffffffu / (unsigned)(heads & 7) : 0u;
+    o.even = n_seg + 2 <= EVEN_MAX;
+    o.by_length = N / EVEN_LONG >= n_seg;
+    if (o.even) o.grid = o.n_blk * heads;
     return o;
 }
 

@@ -273,6 +273,18 @@ def test_attention(lens, H, G, tail, D):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,G,tail,lead", [([900, 3, 1300, 0, 512, 700], 9, 3, 140, 0), ([513, 1500, 640], 3, 1, 0, 200), ([700] * 3, 10, 2, 1, 1),
+                                                ([17] * 62, 9, 9, 3, 0), ([17] * 63, 9, 9, 3, 0), ([130, 1] * 31, 2, 1, 0, 5),
+                                                ([2100], 3, 3, 0, 300), ([0, 0, 0], 2, 2, 300, 0)])
+def test_attention_every_order_of_blocks(lens, H, G, tail, lead, D):
+    """By length, by number (up to 62 sequences) and by groups; heads in eights and what is left of them; nothing but gaps."""
+    q, k, v, cu, cut, dout, _ = attention_inputs(len(lens) + H + D, lens, H, G, D, tail, lead)
+    got = check_attention(q, k, v, cu, cut, dout)
+    for t in (got[0],) + got[2:]:
+        assert not t[:lead].any() and not t[cu[-1]:].any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("masked", [False, True])
 def test_attention_short_sequences_have_an_exact_delta(D, masked):
     """dq and dk of sequences of one tile: what the rounding of out would leave in delta (all of dq and dk, for one token,
