@@ -15,6 +15,8 @@
 // second product is read from the same row-major tile with ds_read_b64_tr_b16: the LDS image's 16-byte chunks are
 // XOR-swizzled by a function of the row that keeps both the row reads and the transposed reads free of bank conflicts.
 //
+// Calls with no more blocks of 128 rows than CUs run smaller blocks, whose four waves share the other side ("few rows" below).
+//
 // The backward pass is two kernels, each with one owner for every output element (no atomics, so the same inputs give the
 // same bits): dQ per query block (three products; it also forms delta), dK / dV per key block (four).
 //
@@ -56,9 +58,9 @@ __device__ __forceinline__ int swz(int r) {
 
 // LDS-DMA of one tile: a wave moves pieces of 1 KiB (64 lanes x 16 bytes, LDS side linear, swizzle on the source address).
 // Rows past `rows` are out of the descriptor's range and land as zeros.
-template <int D, int ROWS = TR>
+template <int D, int ROWS = TR, int WAVES = AG_WAVES>
 struct Stage {
-    static constexpr int RB = 2 * D, CPR = D / 8, PIECES = ROWS * RB / 1024 / AG_WAVES;
+    static constexpr int RB = 2 * D, CPR = D / 8, PIECES = ROWS * RB / 1024 / WAVES;
     unsigned off[PIECES];
     unsigned ldb;
     __device__ __forceinline__ void init(int64_t ld, int wave, int lane) {
@@ -222,7 +224,7 @@ __device__ __forceinline__ void store_row(__bf16* row, const f32x16 (&o)[D / 32]
 // XCD's L2, the XCDs together read whole rows of a fused qkv buffer, and sequences of unequal length load all XCDs alike.  Within
 // an XCD four groups advance together: its workgroups go to its shader engines in turn, and a group's block numbers without rows
 // would otherwise fall to the same engines every time (128-token sequences: every second number; forward pass 118 -> 86 us).
-constexpr int AG_BLK = 128;  // rows a workgroup owns
+constexpr int AG_BLK = 128, AG_FEW_BLK = 32;  // rows a workgroup owns
 struct Order {
     int n_blk, chunk, heads, grid;       // chunk: block numbers of an average sequence
     unsigned by_chunk, by_heads;         // reciprocals, see quotient()
@@ -260,11 +262,12 @@ __device__ __forceinline__ int scan64(int v) {  // sum over this lane and those 
     add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
     return v;
 }
+template <int BLK>
 __device__ __forceinline__ bool find_span_even(const Order& od, const int* __restrict__ cu, int n, int N, int& head, Span& s) {
     const int lane = threadIdx.x & 63, b = blockIdx.x;
     auto start = [&](int i) { return i <= 0 ? 0 : i >= n + 2 ? N : min(max(cu[i - 1], 0), N); };
     auto lane_of = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
-    const int from = start(lane), len = max(start(lane + 1) - from, 0), blocks = (len + AG_BLK - 1) / AG_BLK;
+    const int from = start(lane), len = max(start(lane + 1) - from, 0), blocks = (len + BLK - 1) / BLK;
     const bool live = lane >= 1 && lane <= n;
     int before = 0;
     if (!od.by_length || __ballot(live && len != lane_of(len, 1)) == 0) {  // all alike: nothing to order
@@ -291,14 +294,15 @@ __device__ __forceinline__ bool find_span_even(const Order& od, const int* __res
     }
     s.s0 = lane_of(from, o);
     s.len = lane_of(len, o);
-    s.first = blk * AG_BLK;
+    s.first = blk * BLK;
     s.dead = o == 0 || o == n + 1;
     return true;
 }
 // false: no such block (uniform over the workgroup).  Everything here is on the scalar side, and for sequences of about
 // equal length one read of eight offsets settles it (a vector search took 4500 cycles of a 512-token block's 40000).
+template <int BLK = AG_BLK>
 __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict__ cu, int n, int N, int& head, Span& s) {
-    if (od.even) return find_span_even(od, cu, n, N, head, s);
+    if (od.even) return find_span_even<BLK>(od, cu, n, N, head, s);
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;  // blocks go to the XCDs round-robin
     const int four = at >> 2, turn = quotient(four, od.chunk, od.by_chunk), group = (turn * 4 + (at & 3)) * 8 + xcd;
     const int c = quotient(group, od.heads, od.by_heads);
@@ -316,7 +320,7 @@ __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict
         for (int i = 0; i < 8; ++i) v[i] = clamp(cu[g + i]);  // B(g + 1 + i)
 #pragma unroll
         for (int i = 0; i < 7; ++i) {
-            const bool in = v[i] / AG_BLK + g + 1 + i <= b && b < v[i + 1] / AG_BLK + g + 2 + i;
+            const bool in = v[i] / BLK + g + 1 + i <= b && b < v[i + 1] / BLK + g + 2 + i;
             lo = in ? g + 1 + i : lo;
             a = in ? v[i] : a;
             z = in ? v[i + 1] : z;
@@ -327,7 +331,7 @@ __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict
         int hi = n + 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (start(mid) / AG_BLK + mid <= b) lo = mid;
+            if (start(mid) / BLK + mid <= b) lo = mid;
             else hi = mid - 1;
         }
         a = start(lo);
@@ -335,7 +339,7 @@ __device__ __forceinline__ bool find_span(const Order& od, const int* __restrict
     }
     s.s0 = a;
     s.len = max(z - a, 0);
-    const int64_t first = (int64_t)(b - a / AG_BLK - lo) * AG_BLK;
+    const int64_t first = (int64_t)(b - a / BLK - lo) * BLK;
     s.dead = lo == 0 || lo == n + 1;
     s.first = (int)first;
     return first < s.len;
@@ -748,10 +752,346 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
     store_row<D>(ovp, av, 1.f, hi, on);
 }
 
-Order ag_order(int N, int n_seg, int heads) {
+// ---- few rows ------------------------------------------------------------------------------------------------------------
+// Where the blocks of 128 rows do not fill the card, a workgroup owns 32 rows and its four waves take every fourth tile of the
+// other side, each through a ring of its own and without a barrier; at the end their sums are joined in LDS, in the order of
+// the waves.  Four times the workgroups, each a quarter as long; four times the tile loads.  One path for all masks.
+// Forward and backward pass, blocks of 128 rows and this (blocks of 128, us): one sequence of 4096, a head of 64: 35 blocks, 67, 184
+// and 39, 78; 4 heads: 140, 72, 190 and 49, 102; 3 of 2652, 3 heads: 201, 62, 150 and 63, 128; one of 4096, 8 heads: 280, 76, 199 and
+// 85, 183; 12 heads: 420, 92, 248 and 118, 262; heads of 128, 2: 70, 104, 323 and 56, 134; 8: 280, 118, 356 and 181, 449.  3 of 2652,
+// 4 : 1 heads of 128, where only dK dV is short of blocks (67): backward pass 582 and 248.
+
+// Sum of the four waves' accumulators [column 32 t + crow(r, hi)][row on the lane], each times its `mul`, written as bf16 rows.
+// All waves have to be done with `area`.
+template <int D>
+__device__ __forceinline__ void join_rows(float* area, const f32x16 (&acc)[D / 32], float mul, int wave, int lane, __bf16* p,
+                                          int64_t tok, int rows) {
+    float* mine = area + (wave * 32 + (lane & 31)) * (D + 4) + 4 * (lane >> 5);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(f32x4*)(mine + 32 * t + 8 * g) = f32x4{acc[t][4 * g] * mul, acc[t][4 * g + 1] * mul, acc[t][4 * g + 2] * mul, acc[t][4 * g + 3] * mul};
+    __syncthreads();
+    const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * (D / 8);
+#pragma unroll
+    for (int j = 0; j < D / 8; j += 8) {
+        f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll
+        for (int w = 0; w < AG_WAVES; ++w) {
+            const float* src = area + (w * 32 + row) * (D + 4) + col + j;
+            a += *(const f32x4*)src;
+            b += *(const f32x4*)(src + 4);
+        }
+        if (row < rows)
+            *(u32x4*)(p + row * tok + col + j) = u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
+    }
+}
+
+// Tiles wave, wave + 4, ... of 32 keys, through the wave's own ring (2 slots of K and V).
+template <int D, typename F>
+__device__ __forceinline__ void for_own_tiles(const View& k, const View& v, const unsigned char* mask, const Span& sp, int kvh,
+                                              char* ring, float (*bias)[32], int wave, int lane, F tile) {
+    constexpr int TILE = 32 * 2 * D, SLOT = 2 * TILE;
+    const __bf16* kb = k.p + sp.s0 * k.tok + kvh * k.head;
+    const __bf16* vb = v.p + sp.s0 * v.tok + kvh * v.head;
+    Stage<D, 32, 1> sk, sv;
+    sk.init(k.tok, 0, lane);
+    sv.init(v.tok, 0, lane);
+    const int nt = (sp.len + 31) / 32;
+    auto mask_at = [&](int t) -> unsigned char { return lane < 32 ? mask_byte(mask, sp.s0, t * 32 + lane, sp.len) : 0; };
+    auto stage = [&](int slot, int kt, unsigned long long bits) {
+        sk.go_masked(ring + slot, kb + (int64_t)kt * 32 * k.tok, sp.len - kt * 32, 0, lane, bits);
+        sv.go_masked(ring + slot + TILE, vb + (int64_t)kt * 32 * v.tok, sp.len - kt * 32, 0, lane, bits);
+    };
+    if (wave >= nt) return;
+    unsigned long long bits = __ballot(mask_at(wave) != 0);  // of tile kt
+    unsigned char mb = mask_at(wave + AG_WAVES);             // of tile kt + 4
+    stage(0, wave, bits);
+    for (int kt = wave, i = 0; kt < nt; kt += AG_WAVES, i ^= 1) {
+        const int cur = i * SLOT;
+        if (lane < 32) bias[i][lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the tile has landed, the other slot has been read
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned long long now = bits;
+        bits = __ballot(mb != 0);
+        mb = mask_at(kt + 2 * AG_WAVES);
+        if (kt + AG_WAVES < nt) stage(SLOT - cur, kt + AG_WAVES, bits);
+        if (now != 0) tile(cur, bias[i]);
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_fwd_few_kernel(View q, View k, View v, OutView o,
+                                                                                      float* __restrict__ lse, const int* __restrict__ cu,
+                                                                                      int n_seg, const unsigned char* __restrict__ mask,
+                                                                                      int N, int group, Order od, float c) {
+    constexpr int TILE = 32 * 2 * D, RING = 4 * TILE;
+    __shared__ __attribute__((aligned(1024))) char smem[AG_WAVES * RING];
+    __shared__ __attribute__((aligned(16))) float bias[AG_WAVES][2][32];
+    __shared__ float part[AG_WAVES][2][32];  // reference and sum of each wave's rows
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int head;
+    Span sp;
+    if (!find_span<AG_FEW_BLK>(od, cu, n_seg, N, head, sp)) return;
+    const int row = sp.first + l31;
+    const bool on = row < sp.len;
+    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] = splat16(0.f);
+    if (sp.dead) {
+        if (wave == 0) {
+            store_row<D>(o.p + tok * o.tok + head * o.head, acc, 0.f, hi, on);
+            if (on && hi == 0) lse[(int64_t)head * N + tok] = -INFINITY;
+        }
+        return;
+    }
+    bf16x8 qf[D / 16];
+    {
+        const __bf16* qp = q.p + tok * q.tok + head * q.head + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8*)(qp + ks * 16);
+    }
+    const int koff = row_off<D>(0, l31, hi);
+    TrAddr<D> ta;
+    ta.init(lane);
+    char* ring = smem + wave * RING;
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(ring);
+    float mc = 0.f, l = 0.f;
+    bool fresh = true;
+    for_own_tiles<D>(k, v, mask, sp, head / group, ring, bias[wave], wave, lane, [&](int cur, const float* st) {
+        const f32x16 s = mfma_rows<D>(ring + cur, koff, qf, rows16(st, 0, hi));
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        mx = half_max(mx) * c;
+        // the reference as in the large kernel: from the first tile with keys, and again past 2^16
+        if (fresh || __any(!(mx <= mc + 16.f))) {
+            const float mn = fresh ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mc, mx);
+            const float a = fresh ? 0.f : __builtin_amdgcn_exp2f(mc - mn);
+            mc = mn;
+            fresh = false;
+            l *= a;
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[t][r] *= a;
+        }
+        float e[16], ps = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
+            ps += e[r];
+        }
+        l += ps;
+        const bf16x8 p[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, in the product with V only
+        mfma_tr<D, 0>(acc, ta, lds0 + cur + TILE, p);
+    });
+    l = half_sum(l);
+    if (hi == 0) {
+        part[wave][0][l31] = mc;
+        part[wave][1][l31] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < AG_WAVES; ++w) top = fmaxf(top, part[w][1][l31] == 0.f ? -INFINITY : part[w][0][l31]);
+#pragma unroll
+    for (int w = 0; w < AG_WAVES; ++w) sum += part[w][1][l31] == 0.f ? 0.f : part[w][1][l31] * __builtin_amdgcn_exp2f(part[w][0][l31] - top);
+    const float own = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(mc - top);
+    if (wave == 0 && on && hi == 0) lse[(int64_t)head * N + tok] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * AG_LN2;
+    join_rows<D>((float*)smem, acc, sum > 0.f ? own / sum : sum, wave, lane, o.p + (sp.s0 + sp.first) * o.tok + head * o.head, o.tok,
+                 sp.len - sp.first);
+}
+
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dq_few_kernel(View dout, View q, View k, View v, View o,
+                                                                        const float* __restrict__ lse,
+                                                                        float* __restrict__ delta, OutView dq,
+                                                                        const int* __restrict__ cu, int n_seg,
+                                                                        const unsigned char* __restrict__ mask, int N,
+                                                                        int group, Order od, float scale) {
+    constexpr int TILE = 32 * 2 * D, RING = 4 * TILE;
+    __shared__ __attribute__((aligned(1024))) char smem[AG_WAVES * RING];
+    __shared__ __attribute__((aligned(16))) float bias[AG_WAVES][2][32];
+    __shared__ float part[AG_WAVES][32];
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int head;
+    Span sp;
+    if (!find_span<AG_FEW_BLK>(od, cu, n_seg, N, head, sp)) return;
+    const int row = sp.first + l31;
+    const bool on = row < sp.len;
+    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] = splat16(0.f);
+    if (sp.dead) {
+        if (wave == 0) store_row<D>(dq.p + tok * dq.tok + head * dq.head, acc, 0.f, hi, on);
+        return;
+    }
+    bf16x8 qf[D / 16], gf[D / 16];
+    float dl = 0.f;
+    {
+        const __bf16* qp = q.p + tok * q.tok + head * q.head + hi * 8;
+        const __bf16* gp = dout.p + tok * dout.tok + head * dout.head + hi * 8;
+        const __bf16* xp = o.p + tok * o.tok + head * o.head + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            qf[ks] = *(const bf16x8*)(qp + ks * 16);
+            gf[ks] = *(const bf16x8*)(gp + ks * 16);
+            const bf16x8 xf = *(const bf16x8*)(xp + ks * 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dl += (float)gf[ks][j] * (float)xf[j];
+        }
+    }
+    f32x16 nd = splat16(-half_sum(dl));
+    const float c = scale * AG_LOG2E;
+    const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;
+    const int koff = row_off<D>(0, l31, hi);
+    TrAddr<D> ta;
+    ta.init(lane);
+    char* ring = smem + wave * RING;
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(ring);
+    float e[16];  // P (dP - delta) of a tile
+    auto products = [&](int cur, const float* st) {
+        const f32x16 s = mfma_rows<D>(ring + cur, koff, qf, rows16(st, 0, hi));
+        const f32x16 dp = mfma_rows<D>(ring + cur + TILE, koff, gf, nd);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
+    };
+    if (sp.len <= TR) {  // delta without the rounding of out, as in the large kernel
+        float more = 0.f;
+        for_own_tiles<D>(k, v, mask, sp, head / group, ring, bias[wave], wave, lane, [&](int cur, const float* st) {
+            products(cur, st);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) more += e[r];
+        });
+        more = half_sum(more);
+        if (hi == 0) part[wave][l31] = more;
+        __syncthreads();
+        more = 0.f;
+#pragma unroll
+        for (int w = 0; w < AG_WAVES; ++w) more += part[w][l31];
+        nd = splat16(nd[0] - more);
+    }
+    if (wave == 0 && on && hi == 0) delta[(int64_t)head * N + tok] = -nd[0];
+    for_own_tiles<D>(k, v, mask, sp, head / group, ring, bias[wave], wave, lane, [&](int cur, const float* st) {
+        products(cur, st);
+        const bf16x8 ds[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with K
+        mfma_tr<D, 0>(acc, ta, lds0 + cur, ds);
+    });
+    __syncthreads();
+    join_rows<D>((float*)smem, acc, scale, wave, lane, dq.p + (sp.s0 + sp.first) * dq.tok + head * dq.head, dq.tok, sp.len - sp.first);
+}
+
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dkdv_few_kernel(View dout, View q, View k, View v,
+                                                                      const float* __restrict__ lse,
+                                                                      const float* __restrict__ delta, OutView dk,
+                                                                      OutView dv, const int* __restrict__ cu, int n_seg,
+                                                                      const unsigned char* __restrict__ mask, int N,
+                                                                      int group, Order od, float scale) {
+    constexpr int TILE = 32 * 2 * D, SLOT = 2 * TILE, RING = 2 * SLOT;
+    __shared__ __attribute__((aligned(1024))) char smem[AG_WAVES * RING];
+    __shared__ __attribute__((aligned(16))) float stat[AG_WAVES][2][2][32];  // slot, (-lse / scale, -delta), row of the tile
+    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int kvh;
+    Span sp;
+    if (!find_span<AG_FEW_BLK>(od, cu, n_seg, N, kvh, sp)) return;
+    const int row = sp.first + l31;
+    const bool on = row < sp.len;
+    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
+    f32x16 ak[D / 32], av[D / 32];
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = splat16(0.f);
+    const bool live = on && !sp.dead && (!mask || mask[tok]);
+    if (!__any(live)) {  // no key of the block takes part; every wave has the same rows
+        if (wave == 0) {
+            store_row<D>(dk.p + tok * dk.tok + kvh * dk.head, ak, 0.f, hi, on);
+            store_row<D>(dv.p + tok * dv.tok + kvh * dv.head, av, 0.f, hi, on);
+        }
+        return;
+    }
+    bf16x8 kf[D / 16], vf[D / 16];  // zero rows for keys that take no part: their columns are computed and not used
+    {
+        const __bf16* kp = k.p + tok * k.tok + kvh * k.head + hi * 8;
+        const __bf16* vp = v.p + tok * v.tok + kvh * v.head + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            u32x4 a = u32x4{0u, 0u, 0u, 0u}, b = a;
+            if (live) {
+                a = *(const u32x4*)(kp + ks * 16);
+                b = *(const u32x4*)(vp + ks * 16);
+            }
+            kf[ks] = __builtin_bit_cast(bf16x8, a);
+            vf[ks] = __builtin_bit_cast(bf16x8, b);
+        }
+    }
+    Stage<D, 32, 1> sq, sg;
+    sq.init(q.tok, 0, lane);
+    sg.init(dout.tok, 0, lane);
+    const int nt = (sp.len + 31) / 32;  // query tiles per head of the group
+    const int total = nt * group;
+    const float inv_scale = 1.0f / scale;
+    char* ring = smem + wave * RING;
+    float next = 0.f;
+    int gq = 0, qt = wave;  // head of the group and tile that stage() takes next
+    auto stage = [&](int slot) {
+        for (; qt >= nt; qt -= nt) ++gq;
+        const int left = sp.len - qt * 32, head = kvh * group + gq;
+        const int64_t t0 = sp.s0 + (int64_t)qt * 32;
+        sq.go(ring + slot, q.p + t0 * q.tok + head * q.head, left, 0);
+        sg.go(ring + slot + TILE, dout.p + t0 * dout.tok + head * dout.head, left, 0);
+        // lanes 0 .. 31: lse, 32 .. 63: delta.  Rows past the end get probability 2^-inf = 0
+        const float* src = (hi ? delta : lse) + (int64_t)head * N + t0;
+        const float x = l31 < left ? src[l31] : hi ? 0.f : INFINITY;
+        next = hi ? -x : -x * inv_scale;
+        qt += AG_WAVES;
+    };
+    const int koff = row_off<D>(0, l31, hi);
+    TrAddr<D> ta;
+    ta.init(lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(ring);
+    const float c = scale * AG_LOG2E;
+    if (wave < total) stage(0);
+    for (int i = wave, j = 0; i < total; i += AG_WAVES, j ^= 1) {
+        const int cur = j * SLOT;
+        stat[wave][j][hi][l31] = next;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + AG_WAVES < total) stage(SLOT - cur);
+        const f32x16 s = mfma_rows<D>(ring + cur, koff, kf, rows16(stat[wave][j][0], 0, hi));         // Q K^T - lse / scale
+        const f32x16 dp = mfma_rows<D>(ring + cur + TILE, koff, vf, rows16(stat[wave][j][1], 0, hi));  // dO V^T - delta
+        float e[16], f[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            e[r] = __builtin_amdgcn_exp2f(s[r] * c);
+            f[r] = e[r] * dp[r];
+        }
+        // 2^-8 relative at most, for the products with dO and Q
+        const bf16x8 p[2] = {pack8(e), pack8(e + 8)}, ds[2] = {pack8(f), pack8(f + 8)};
+        mfma_tr<D, 0>(av, ta, lds0 + cur + TILE, p);
+        mfma_tr<D, 0>(ak, ta, lds0 + cur, ds);
+    }
+    if (!live) {
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = splat16(0.f);
+    }
+    __syncthreads();
+    const int64_t first = sp.s0 + sp.first;
+    join_rows<D>((float*)smem, ak, scale, wave, lane, dk.p + first * dk.tok + kvh * dk.head, dk.tok, sp.len - sp.first);
+    __syncthreads();
+    join_rows<D>((float*)smem, av, 1.f, wave, lane, dv.p + first * dv.tok + kvh * dv.head, dv.tok, sp.len - sp.first);
+}
+
+Order ag_order(int N, int n_seg, int heads, int blk = AG_BLK) {
     Order o;
-    o.n_blk = N / AG_BLK + n_seg + 2;
-    o.chunk = N / AG_BLK / (n_seg > 0 ? n_seg : 1) + 1;
+    o.n_blk = N / blk + n_seg + 2;
+    o.chunk = N / blk / (n_seg > 0 ? n_seg : 1) + 1;
     o.heads = heads;
     const int groups = (o.n_blk + o.chunk - 1) / o.chunk * heads;
     o.grid = (groups + 31) / 32 * 32 * o.chunk;
@@ -765,6 +1105,8 @@ Order ag_order(int N, int n_seg, int heads) {
     if (o.even) o.grid = o.n_blk * heads;
     return o;
 }
+// No more blocks of 128 rows than CUs.
+bool ag_few(int N, int n_seg, int heads) { return (N / AG_BLK + n_seg + 2) * (long long)heads <= 256; }
 
 bool ag_strides(const void* p, const int64_t* st, int D) {
     // 16-byte rows; a tile's offsets (64 rows) stay inside the 31 bits of a buffer descriptor
@@ -797,9 +1139,11 @@ extern "C" int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v,
     const View vq{(const __bf16*)q, strides[0], strides[1]}, vk{(const __bf16*)k, strides[2], strides[3]}, vv{(const __bf16*)v, strides[4], strides[5]};
     const OutView vo{(__bf16*)out, strides[6], strides[7]};
     const int group = n_heads / n_kv_heads;
-    const Order od = ag_order(n_tokens, n_segments, n_heads);
-    auto* kern = head_dim == 64 ? (key_mask ? attn_fwd_lse_kernel<64, true> : attn_fwd_lse_kernel<64, false>)
-                                : (key_mask ? attn_fwd_lse_kernel<128, true> : attn_fwd_lse_kernel<128, false>);
+    const bool few = ag_few(n_tokens, n_segments, n_heads);
+    const Order od = ag_order(n_tokens, n_segments, n_heads, few ? AG_FEW_BLK : AG_BLK);
+    auto* kern = few             ? (head_dim == 64 ? attn_fwd_few_kernel<64> : attn_fwd_few_kernel<128>)
+                 : head_dim == 64 ? (key_mask ? attn_fwd_lse_kernel<64, true> : attn_fwd_lse_kernel<64, false>)
+                                  : (key_mask ? attn_fwd_lse_kernel<128, true> : attn_fwd_lse_kernel<128, false>);
     hipLaunchKernelGGL(kern, dim3(od.grid), dim3(AG_WAVES * 64), 0, (hipStream_t)stream, vq, vk, vv, vo, lse, cu_seqlens, n_segments,
                        key_mask, n_tokens, group, od, scale * AG_LOG2E);
     ESMK_CHECK_LAUNCH("esmk_attn_varlen_fwd");
@@ -827,14 +1171,18 @@ extern "C" int esmk_attn_varlen_bwd(const void* dout, const void* q, const void*
     auto in = [&](int i) { return View{(const __bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
     auto ov = [&](int i) { return OutView{(__bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
     const int group = n_heads / n_kv_heads;
-    const Order oq = ag_order(n_tokens, n_segments, n_heads), ok = ag_order(n_tokens, n_segments, n_kv_heads);
+    const bool few_q = ag_few(n_tokens, n_segments, n_heads), few_k = ag_few(n_tokens, n_segments, n_kv_heads);
+    const Order oq = ag_order(n_tokens, n_segments, n_heads, few_q ? AG_FEW_BLK : AG_BLK);
+    const Order ok = ag_order(n_tokens, n_segments, n_kv_heads, few_k ? AG_FEW_BLK : AG_BLK);
     float* delta = (float*)workspace;
     hipStream_t s = (hipStream_t)stream;
-    auto* kq = head_dim == 64 ? (key_mask ? attn_bwd_dq_kernel<64, true> : attn_bwd_dq_kernel<64, false>)
+    auto* kq = few_q           ? (head_dim == 64 ? attn_bwd_dq_few_kernel<64> : attn_bwd_dq_few_kernel<128>)
+               : head_dim == 64 ? (key_mask ? attn_bwd_dq_kernel<64, true> : attn_bwd_dq_kernel<64, false>)
                               : (key_mask ? attn_bwd_dq_kernel<128, true> : attn_bwd_dq_kernel<128, false>);
     hipLaunchKernelGGL(kq, dim3(oq.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), in(4), lse, delta, ov(5),
                        cu_seqlens, n_segments, key_mask, n_tokens, group, oq, scale);
-    auto* kk = head_dim == 64 ? attn_bwd_dkdv_kernel<64> : attn_bwd_dkdv_kernel<128>;
+    auto* kk = few_k ? (head_dim == 64 ? attn_bwd_dkdv_few_kernel<64> : attn_bwd_dkdv_few_kernel<128>)
+                     : (head_dim == 64 ? attn_bwd_dkdv_kernel<64> : attn_bwd_dkdv_kernel<128>);
     hipLaunchKernelGGL(kk, dim3(ok.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), lse, delta, ov(6), ov(7),
                        cu_seqlens, n_segments, key_mask, n_tokens, group, ok, scale);
     ESMK_CHECK_LAUNCH("esmk_attn_varlen_bwd");

@@ -251,16 +251,27 @@ def attention_all(q, k, v, cu, dout, scale=None, mask=None):
     return (out, lse) + T().attention_varlen_backward(dout, q, k, v, out, lse, cu, scale, mask)
 
 
-def check_attention(q, k, v, cu, cut, dout, scale=None, mask=None):
-    got = attention_all(q, k, v, cut, dout, scale, mask)
-    want, tol = attention_oracle(q, k, v, cu, scale or q.shape[2] ** -0.5, mask, dout)
+def copies(N, n, G):
+    """How often the heads have to be repeated for more than 256 blocks of 128 rows: fewer go other ways through the kernels."""
+    return 256 // ((N // 128 + n + 2) * G) + 1
+
+
+def check_attention(q, k, v, cu, cut, dout, scale=None, mask=None, short=False):
+    """Few heads, and the same heads so often that the kernels for many blocks run, against one oracle."""
+    want, tol = attention_oracle(q, k, v, cu, scale or q.shape[2] ** -0.5, mask, dout, short)
     none = want[1] == -math.inf
-    assert torch.equal(got[1] == -math.inf, none)
-    lse = got[1].masked_fill(none, 0.0)
     want = (want[0], want[1].masked_fill(none, 0.0)) + want[2:]
-    for a, b, t, n in zip((got[0], lse) + got[2:], want, tol, ("out", "lse", "dq", "dk", "dv")):
-        within(a, b, t, n)
-    return got
+    first = None
+    for r in (1, copies(len(q), len(cu) - 1, k.shape[1])):
+        got = attention_all(*(t.repeat(1, r, 1) if r > 1 else t for t in (q, k, v)), cut, dout.repeat(1, r, 1), scale, mask)
+        first = first or got
+        lse = got[1].view(r, *none.shape)
+        assert torch.equal(lse == -math.inf, none.expand_as(lse))
+        got = tuple(t.view(len(q), r, -1, q.shape[2]).transpose(0, 1) for t in got[:1] + got[2:])
+        for a, b, t, n in zip((got[0], lse.masked_fill(none, 0.0)) + got[1:], want, tol, ("out", "lse", "dq", "dk", "dv")):
+            within(a, b.expand_as(a), t, f"{n}, {r} copies")
+            assert torch.equal(a[0], a[-1])
+    return first
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -275,7 +286,7 @@ def test_attention(lens, H, G, tail, D):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("lens,H,G,tail,lead", [([900, 3, 1300, 0, 512, 700], 9, 3, 140, 0), ([513, 1500, 640], 3, 1, 0, 200), ([700] * 3, 10, 2, 1, 1),
                                                 ([17] * 62, 9, 9, 3, 0), ([17] * 63, 9, 9, 3, 0), ([130, 1] * 31, 2, 1, 0, 5),
-                                                ([2100], 3, 3, 0, 300), ([0, 0, 0], 2, 2, 300, 0)])
+                                                ([2100], 3, 3, 0, 300), ([0, 0, 0], 2, 2, 300, 0), ([300, 90], 64, 1, 5, 0)])
 def test_attention_every_order_of_blocks(lens, H, G, tail, lead, D):
     """By length, by number (up to 62 sequences) and by groups; heads in eights and what is left of them; nothing but gaps."""
     q, k, v, cu, cut, dout, _ = attention_inputs(len(lens) + H + D, lens, H, G, D, tail, lead)
@@ -294,10 +305,7 @@ def test_attention_short_sequences_have_an_exact_delta(D, masked):
     if masked:
         mask = torch.rand(len(q), generator=g, device="cuda") > 0.2
         mask[cu[2]:cu[3]] = False
-    got = attention_all(q, k, v, cut, dout, mask=mask)
-    want, tol = attention_oracle(q, k, v, cu, D ** -0.5, mask, dout, short=True)
-    for a, b, t, n in zip(got[2:], want[2:], tol[2:], ("dq", "dk", "dv")):
-        within(a, b, t, n)
+    check_attention(q, k, v, cu, cut, dout, mask=mask, short=True)
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -320,6 +328,11 @@ def test_attention_key_mask(D):
         t[:5], t[cu[-1]:] = math.nan, math.nan
     d2[cu[1]:cu[2]] = math.inf  # queries without a key
     for a, b in zip(got, attention_all(q2, k2, v2, cut, d2, mask=mask)):
+        assert torch.equal(a, b)
+    many = lambda *ts: [t.repeat(1, copies(len(q), 4, 2), 1) for t in ts]
+    q3, k3, v3, d3 = many(q, k, v, dout)
+    q4, k4, v4, d4 = many(q2, k2, v2, d2)
+    for a, b in zip(attention_all(q3, k3, v3, cut, d3, mask=mask), attention_all(q4, k4, v4, cut, d4, mask=mask)):
         assert torch.equal(a, b)
 
 
@@ -365,9 +378,11 @@ def test_attention_layouts():
     far.copy_(randn(gen(2), N, 3, 64))
     cut = torch.tensor([0, 150, N], dtype=torch.int32, device="cuda")
     near = far.contiguous()
-    d = dout.new_ones(N, 1, 64)
-    for a, b in zip(attention_all(far[:, :1], far[:, 1:2], far[:, 2:], cut, d), attention_all(near[:, :1], near[:, 1:2], near[:, 2:], cut, d)):
-        assert torch.equal(a, b)
+    for r in (1, copies(N, 2, 1)):  # heads that are all the same memory
+        d = dout.new_ones(N, r, 64)
+        at = lambda t, i: t[:, i:i + 1].expand(-1, r, -1)
+        for a, b in zip(attention_all(at(far, 0), at(far, 1), at(far, 2), cut, d), attention_all(at(near, 0), at(near, 1), at(near, 2), cut, d)):
+            assert torch.equal(a, b)
 
 
 def test_attention_more_than_2_31_elements():
