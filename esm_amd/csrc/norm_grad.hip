@@ -300,6 +300,187 @@ __global__ __launch_bounds__(ng_threads(WPR)) void norm_bwd_kernel(const T* __re
     }
 }
 
+// ---- narrow rows ----------------------------------------------------------------------------------------------------------
+// Up to 256 elements: 16 lanes per row, four rows in a wave.  A wave per row spends about 150 instructions on one whatever its
+// width: 32768 x 64 bf16 forward and backward 9.6, 12.2 us that way and 4.8, 7.6 this way; x 77 fp32 10.6, 15.5 and 6.6, 9.0;
+// x 256 bf16 10.3, 13.4 and 7.7, 12.8.  The 16 rows of a workgroup go through one buffer descriptor; lanes past the end of a row,
+// and rows past the last, are addressed out of its range.
+constexpr int NG_NARROW = 256, NG_NARROW_ROWS = 16;
+constexpr int NG_OUT = 0x7ffffff0;
+
+__device__ __forceinline__ float sum16(float v) {
+    auto step = [&](auto ctrl) { v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false)); };
+    step(std::integral_constant<int, 0xB1>{});   // lane ^ 1
+    step(std::integral_constant<int, 0x4E>{});   // lane ^ 2
+    step(std::integral_constant<int, 0x141>{});  // mirrored in 8
+    step(std::integral_constant<int, 0x140>{});  // mirrored in 16
+    return v;
+}
+// the same column of a wave's four rows
+__device__ __forceinline__ float sum_rows4(float v) {
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// Rows row0 .. row0 + 15 of a tensor, as far as they exist; a lane's elements start at its column.
+template <typename T, int VEC, int NV>
+struct NgRows {
+    int off[NV];  // bytes from the first row
+    int ld;       // bytes
+    __device__ __forceinline__ NgRows(int64_t ld_, int slot, int sub, int d) : ld((int)(ld_ * (int)sizeof(T))) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (sub + i * 16) * VEC;
+            off[i] = c < d ? slot * ld + c * (int)sizeof(T) : NG_OUT;
+        }
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(const void* p, int row0, int M, int d) const {
+        const int rows = min(M - row0, NG_NARROW_ROWS);  // below 1: none
+        return ng_row((const char*)p + (int64_t)(rows > 0 ? row0 : 0) * ld, rows > 0 ? (rows - 1) * ld + d * (int)sizeof(T) : 0);
+    }
+};
+
+template <typename T, int VEC, int NV>
+__global__ __launch_bounds__(256) void norm_fwd_narrow_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
+                                                              const float* __restrict__ beta, T* __restrict__ y,
+                                                              float* __restrict__ stats, int M, int d, float eps) {
+    const int sub = threadIdx.x & 15, slot = threadIdx.x >> 4, stride = gridDim.x * NG_NARROW_ROWS;
+    const float inv_d = 1.0f / (float)d;
+    const NgRows<T, VEC, NV> rx(ldx, slot, sub, d), ry(d, slot, sub, d);
+    NgRaw<T, VEC> raw[NV];
+    auto load = [&](int row0) {
+        const __amdgpu_buffer_rsrc_t r = rx.at(x, row0, M, d);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = ng_load<T, VEC>(r, rx.off[i]);
+    };
+    int row0 = blockIdx.x * NG_NARROW_ROWS;
+    load(row0);
+    __builtin_amdgcn_sched_barrier(0);
+    float w[NV][VEC], b[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        ng_param<VEC>(gamma, d, (sub + i * 16) * VEC, w[i]);
+        ng_param<VEC>(beta, d, (sub + i * 16) * VEC, b[i]);
+    }
+    for (; row0 < M; row0 += stride) {
+        float v[NV][VEC], sum = 0.f, sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            ng_unpack(raw[i], v[i]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += v[i][e];
+        }
+        load(row0 + stride);
+        const float mean = sum16(sum) * inv_d;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[i][e] = rx.off[i] != NG_OUT ? v[i][e] - mean : 0.f;
+                sq += v[i][e] * v[i][e];
+            }
+        const float rstd = 1.0f / sqrtf(sum16(sq) * inv_d + eps);
+        if (sub == 0 && row0 + slot < M) *(f32x2*)(stats + 2 * (int64_t)(row0 + slot)) = f32x2{mean, rstd};
+        const __amdgpu_buffer_rsrc_t r = ry.at(y, row0, M, d);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = v[i][e] * rstd * w[i][e] + b[i][e];
+            ng_store<T, VEC>(r, ry.off[i], o);
+        }
+    }
+}
+
+template <typename T, int VEC, int NV>
+__global__ __launch_bounds__(256) void norm_bwd_narrow_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+                                                              int64_t ldx, const float* __restrict__ gamma,
+                                                              const float* __restrict__ stats, T* __restrict__ dx,
+                                                              float* __restrict__ pg, float* __restrict__ pb, int M, int d) {
+    __shared__ float part[3][2][NG_NARROW];
+    const int sub = threadIdx.x & 15, slot = threadIdx.x >> 4, stride = gridDim.x * NG_NARROW_ROWS;
+    const float inv_d = 1.0f / (float)d;
+    const NgRows<T, VEC, NV> rx(ldx, slot, sub, d), rg(lddy, slot, sub, d), ro(d, slot, sub, d);
+    NgRaw<T, VEC> raw_x[NV], raw_g[NV];
+    f32x2 st;
+    auto load = [&](int row0) {
+        const __amdgpu_buffer_rsrc_t a = rx.at(x, row0, M, d), b = rg.at(dy, row0, M, d);
+        st = *(const f32x2*)(stats + 2 * (int64_t)min(row0 + slot, M - 1));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            raw_x[i] = ng_load<T, VEC>(a, rx.off[i]);
+            raw_g[i] = ng_load<T, VEC>(b, rg.off[i]);
+        }
+    };
+    int row0 = blockIdx.x * NG_NARROW_ROWS;
+    load(row0);
+    __builtin_amdgcn_sched_barrier(0);
+    float w[NV][VEC], ag[NV][VEC], ab[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        ng_param<VEC>(gamma, d, (sub + i * 16) * VEC, w[i]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) ag[i][e] = ab[i][e] = 0.f;
+    }
+    for (; row0 < M; row0 += stride) {
+        float h[NV][VEC], g[NV][VEC], c1 = 0.f, c2 = 0.f;
+        const bool on = row0 + slot < M;
+        const float mean = on ? st[0] : 0.f, rs = on ? st[1] : 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            ng_unpack(raw_x[i], h[i]);  // past the end of the row, and in a row past the last, dy reads as zero
+            ng_unpack(raw_g[i], g[i]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                h[i][e] = (h[i][e] - mean) * rs;
+                ag[i][e] += g[i][e] * h[i][e];
+                ab[i][e] += g[i][e];
+                g[i][e] *= w[i][e];
+                c1 += g[i][e];
+                c2 += g[i][e] * h[i][e];
+            }
+        }
+        load(row0 + stride);
+        c1 = sum16(c1) * inv_d;
+        c2 = sum16(c2) * inv_d;
+        const __amdgpu_buffer_rsrc_t r = ro.at(dx, row0, M, d);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = (g[i][e] - c1 - h[i][e] * c2) * rs;
+            ng_store<T, VEC>(r, ro.off[i], o);
+        }
+    }
+    if (!pg && !pb) return;
+    const int wave = threadIdx.x >> 6;
+    const bool first = (threadIdx.x & 63) < 16;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            ag[i][e] = sum_rows4(ag[i][e]);
+            ab[i][e] = sum_rows4(ab[i][e]);
+            const int c = (sub + i * 16) * VEC + e;
+            if (wave > 0 && first && c < d) {
+                part[wave - 1][0][c] = ag[i][e];
+                part[wave - 1][1][c] = ab[i][e];
+            }
+        }
+    __syncthreads();
+    if (wave > 0 || !first) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int c = (sub + i * 16) * VEC + e;
+            if (c >= d) continue;
+            if (pg) pg[(int64_t)blockIdx.x * d + c] = ag[i][e] + part[0][0][c] + part[1][0][c] + part[2][0][c];
+            if (pb) pb[(int64_t)blockIdx.x * d + c] = ab[i][e] + part[0][1][c] + part[1][1][c] + part[2][1][c];
+        }
+}
+
 // Column sums of the G partial rows: 32 columns x 32 groups of rows per workgroup, then the groups in order.  A few
 // microseconds of latency: a group's rows are requested eight at a time.
 __global__ __launch_bounds__(1024) void norm_grad_reduce_kernel(const float* __restrict__ pg, const float* __restrict__ pb,
@@ -337,10 +518,10 @@ __global__ void norm_grad_zero_kernel(float* a, float* b, int d) {
 int ng_waves(int d) { return d <= 1536 ? 1 : d <= 2 * 1536 ? 2 : d <= 4 * 1536 ? 4 : 8; }
 int ng_rows(int wpr) { return wpr == 8 ? 1 : 4 / wpr; }
 // Workgroups of the backward pass: two per CU hold enough loads in flight, and more of them only add partial rows; at
-// small M a row slot sees at least four rows.
+// small M a row slot sees at least four rows (two narrow ones).
 int ng_groups(int M, int d) {
-    const int rows = ng_rows(ng_waves(d));
-    const int want = (M + 4 * rows - 1) / (4 * rows);
+    const int rows = d <= NG_NARROW ? 2 * NG_NARROW_ROWS : 4 * ng_rows(ng_waves(d));
+    const int want = (M + rows - 1) / rows;
     return want < NG_MAX_GROUPS ? want : NG_MAX_GROUPS;
 }
 
@@ -364,6 +545,15 @@ bool ng_dispatch(int d, F f) {
     return false;
 }
 
+// d <= NG_NARROW: f(constant<VEC>, constant<NV>)
+template <int VEC, typename F>
+void ng_narrow_dispatch(int d, F f) {
+    if (d <= 128) f(std::integral_constant<int, VEC>{}, std::integral_constant<int, 8 / VEC>{});
+    else f(std::integral_constant<int, VEC>{}, std::integral_constant<int, 16 / VEC>{});
+}
+// The offsets of 16 rows have to fit a buffer descriptor.
+bool ng_narrow(int d, int64_t ld, int size) { return d <= NG_NARROW && ld * size < (1LL << 27); }
+
 bool ng_wide(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15) == 0 && (ld * size) % 16 == 0; }
 
 template <typename T>
@@ -377,6 +567,18 @@ int norm_fwd(const T* x, int64_t ldx, const float* gamma, const float* beta, T* 
         return true;
     };
     const bool wide = ng_wide(x, ldx, sizeof(T)) && ng_wide(y, d, sizeof(T));
+    if (ng_narrow(d, ldx, sizeof(T))) {
+        auto narrow = [&](auto vec, auto nv) {
+            constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
+            const int want = (M + NG_NARROW_ROWS - 1) / NG_NARROW_ROWS;
+            hipLaunchKernelGGL((norm_fwd_narrow_kernel<T, V, N>), dim3(want < NG_FWD_GROUPS ? want : NG_FWD_GROUPS), dim3(256), 0, s,
+                               x, ldx, gamma, beta, y, stats, M, d, eps);
+        };
+        if (wide) ng_narrow_dispatch<NgVec<T>::N>(d, narrow);
+        else ng_narrow_dispatch<1>(d, narrow);
+        ESMK_CHECK_LAUNCH("esmk_layernorm_fwd");
+        return ESMK_OK;
+    }
     if (!(wide ? ng_dispatch<T, NgVec<T>::N>(d, go) : ng_dispatch<T, 1>(d, go)))
         ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "esmk_layernorm_fwd: d=%d", d);
     ESMK_CHECK_LAUNCH("esmk_layernorm_fwd");
@@ -398,7 +600,14 @@ int norm_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const float* ga
         return true;
     };
     const bool wide = ng_wide(x, ldx, sizeof(T)) && ng_wide(dy, lddy, sizeof(T)) && ng_wide(dx, d, sizeof(T));
-    if (!(wide ? ng_dispatch<T, NgVec<T>::N>(d, go) : ng_dispatch<T, 1>(d, go)))
+    auto narrow = [&](auto vec, auto nv) {
+        constexpr int V = decltype(vec)::value, N = decltype(nv)::value;
+        hipLaunchKernelGGL((norm_bwd_narrow_kernel<T, V, N>), dim3(G), dim3(256), 0, s, dy, lddy, x, ldx, gamma, stats, dx, pg, pb, M, d);
+    };
+    if (ng_narrow(d, ldx, sizeof(T)) && ng_narrow(d, lddy, sizeof(T))) {
+        if (wide) ng_narrow_dispatch<NgVec<T>::N>(d, narrow);
+        else ng_narrow_dispatch<1>(d, narrow);
+    } else if (!(wide ? ng_dispatch<T, NgVec<T>::N>(d, go) : ng_dispatch<T, 1>(d, go)))
         ESMK_FAIL(ESMK_ERR_UNSUPPORTED, "esmk_layernorm_bwd: d=%d", d);
     if (G > 1 && (dgamma || dbeta))
         hipLaunchKernelGGL(norm_grad_reduce_kernel, dim3((d + 31) / 32, 2), dim3(1024), 0, s, pg, pb, dgamma, dbeta, G, d);

@@ -72,7 +72,8 @@ def norm_oracle(x, w, b, dy, eps=1e-5):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,d", [(1, 1), (2, 3), (5, 64), (17, 65), (66, 960), (301, 1152), (130, 1281), (1030, 512),
-                                    (37, 2560), (33, 1537), (9, 4097), (7, 6145), (3, 12288), (4099, 33)])
+                                    (37, 2560), (33, 1537), (9, 4097), (7, 6145), (3, 12288), (4099, 33), (700, 256), (33, 255),
+                                    (2049, 136), (5000, 7), (70, 129), (40000, 72), (129, 257)])
 def test_layer_norm(rows, d, dtype):
     g = gen(rows * 31 + d)
     x = (randn(g, rows, d) * 2 + 0.5).to(dtype)
@@ -120,16 +121,21 @@ def test_layer_norm_no_rows_gives_zero_parameter_gradients():
 def test_layer_norm_far_rows():
     """Row offsets past 2^32 bytes."""
     big = torch.empty(300 * 2 ** 23, dtype=torch.bfloat16, device="cuda")
-    x = big.as_strided((300, 64), (2 ** 23, 1))
-    g = gen(3)
-    x.copy_(randn(g, 300, 64))
-    w, dy = 1 + 0.1 * randn(g, 64), randn(g, 300, 64).bfloat16()
-    y, st = T().layer_norm_forward(x, w)
-    got = (y,) + T().layer_norm_backward(dy, x, w, st)
-    xc = x.contiguous()
-    y2, st2 = T().layer_norm_forward(xc, w)
-    for a, b in zip(got, (y2,) + T().layer_norm_backward(dy, xc, w, st2)):
-        assert torch.equal(a, b)
+    for rows, ld, d in ((300, 2 ** 23, 64), (300, 2 ** 23, 320), (37, 2 ** 26, 64)):  # the last: strides that 16 rows cannot share
+        x = big.as_strided((rows, d), (ld, 1))
+        g = gen(3)
+        x.copy_(randn(g, rows, d))
+        w, dy = 1 + 0.1 * randn(g, d), randn(g, rows, d).bfloat16()
+        y, st = T().layer_norm_forward(x, w)
+        got = (y,) + T().layer_norm_backward(dy, x, w, st)
+        xc = x.contiguous()
+        want, tol = norm_oracle(xc, w, None, dy)
+        for a, b, t in zip(got, want, tol):
+            within(a, b, t, "far rows")
+        if ld < 2 ** 26:
+            y2, st2 = T().layer_norm_forward(xc, w)
+            for a, b in zip(got, (y2,) + T().layer_norm_backward(dy, xc, w, st2)):
+                assert torch.equal(a, b)
 
 
 def test_layer_norm_more_than_2_31_elements():
