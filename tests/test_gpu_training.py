@@ -73,7 +73,8 @@ def norm_oracle(x, w, b, dy, eps=1e-5):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,d", [(1, 1), (2, 3), (5, 64), (17, 65), (66, 960), (301, 1152), (130, 1281), (1030, 512),
                                     (37, 2560), (33, 1537), (9, 4097), (7, 6145), (3, 12288), (4099, 33), (700, 256), (33, 255),
-                                    (2049, 136), (5000, 7), (70, 129), (40000, 72), (129, 257)])
+                                    (2049, 136), (5000, 7), (70, 129), (40000, 72), (129, 257), (512, 1152), (513, 1152), (600, 2560),
+                                    (601, 1537), (530, 4097), (520, 6145), (515, 12288), (900, 1281), (512, 12288), (400, 4096)])
 def test_layer_norm(rows, d, dtype):
     g = gen(rows * 31 + d)
     x = (randn(g, rows, d) * 2 + 0.5).to(dtype)

@@ -38,6 +38,7 @@ def test_layernorm_entry_points_refuse():
     refused(bwd(M=2 ** 30 + 1), UNSUPPORTED, "M=1073741825")
     refused(bwd(ws=None), WORKSPACE, "workspace")
     refused(bwd(nb=lib.esmk_layernorm_bwd_workspace_bytes(4096, 64) - 1), WORKSPACE, "workspace")
+    assert lib.esmk_layernorm_bwd_workspace_bytes(512, 12288) == 0 and lib.esmk_layernorm_bwd_workspace_bytes(513, 64) > 0
     assert lib.esmk_layernorm_bwd_workspace_bytes(0, 64) == 0 and lib.esmk_layernorm_bwd_workspace_bytes(4096, 64) > 0
 
 
