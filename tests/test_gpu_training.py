@@ -187,12 +187,13 @@ def test_layer_norm_autograd_and_differences():
 
 # ------------------------------------------------------------------------------------------------ attention
 
-def attention_oracle(q, k, v, cu, scale, mask, dout, short=False):
+def attention_oracle(q, k, v, cu, scale, mask, dout, short=False, rest=False):
     """64-bit (out, lse, dq, dk, dv) and bounds.  Where the kernels round: P to bf16 before P V and P^T dO (r), dS to bf16
     before dS K and dS^T Q (r), outputs (r); delta uses the rounded out.  fp32: a score has D products (D u of their
     magnitudes) and moves P by that, relatively; sums over keys or queries L u.  Below the smallest normal number, 2^-126, a
     probability or a result may be flushed to zero: that much is added wherever one enters.  short: sequences of at most 64
-    tokens, where delta is summed again as delta + rowsum(P (dP - delta)) and out's rounding leaves it."""
+    tokens, where delta is summed again as delta + rowsum(P (dP - delta)) and out's rounding leaves it.
+    rest: dS in two bf16 parts, off by r r / 2 of it."""
     r = R[torch.bfloat16]
     N, H, D = q.shape
     G = k.shape[1]
@@ -226,7 +227,7 @@ def attention_oracle(q, k, v, cu, scale, mask, dout, short=False):
             if short:
                 assert L <= 64
                 eDl = ((eP + (L + 32) * U) * P * ((dP - dl).abs() + eDl) + P * eDP).sum(-1, keepdim=True) + 2 * U * dl.abs()
-            eds = P * (eDl + eDP + eP * (dP - dl).abs()) * (1 + r) + r * dS.abs() + TINY * (1 + (dP - dl).abs())  # abs, of the rounded dS
+            eds = P * (eDl + eDP + eP * (dP - dl).abs()) * (1 + r) + r * (r if rest else 1) * dS.abs() + TINY * (1 + (dP - dl).abs())  # abs, of the rounded dS
             n = (L + 32) * U
             o[a:e, h], to[a:e, h] = O, tO
             lse[h, a:e] = ls[:, 0]
@@ -312,7 +313,11 @@ def test_attention_short_sequences_have_an_exact_delta(D, masked):
     if masked:
         mask = torch.rand(len(q), generator=g, device="cuda") > 0.2
         mask[cu[2]:cu[3]] = False
-    check_attention(q, k, v, cu, cut, dout, mask=mask, short=True)
+    got = check_attention(q, k, v, cu, cut, dout, mask=mask, short=True)
+    # few blocks: dS's rounding has a second product, and dq's and dk's own rounding is left
+    want, tol = attention_oracle(q, k, v, cu, D ** -0.5, mask, dout, short=True, rest=True)
+    for a, b, t, n in zip(got[2:4], want[2:4], tol[2:4], ("dq", "dk")):
+        within(a, b, t, n)
 
 
 @pytest.mark.parametrize("D", [64, 128])
