@@ -764,6 +764,34 @@ def test_same_bits_again_on_other_streams_and_in_a_replayed_graph():
                 assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("H,G", [(2, 1), (150, 75)])
+def test_attention_graph_follows_the_offsets(H, G):
+    """The order of the blocks is formed on the GPU: a captured step holds for other offsets, with few blocks and with many."""
+    n = 700
+    sets = []
+    for seed, lens in ((1, [100, 31, 500]), (2, [1, 600, 20]), (3, [0, 0, 700]), (4, [233, 233, 234])):
+        q, k, v, _, cu, dout, g = attention_inputs(seed, lens, H, G, 64, tail=n - sum(lens))
+        sets.append([q.contiguous(), k.contiguous(), v.contiguous(), cu, dout, torch.rand(n, generator=g, device="cuda") > 0.1])
+    step = lambda q, k, v, cu, dout, mask: attention_all(q, k, v, cu, dout) + attention_all(q, k, v, cu, dout, mask=mask)
+    want = [step(*s) for s in sets]
+    bufs = [t.clone() for t in sets[0]]
+    s1 = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        step(*bufs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*bufs)
+    for i in (1, 0, 2, 3, 1):
+        for t, s in zip(bufs, sets[i]):
+            t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want[i]):
+            assert torch.equal(a, b)
+
+
 def test_refusals_name_the_argument():
     t = T()
     x, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
