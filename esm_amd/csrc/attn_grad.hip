@@ -162,7 +162,7 @@ __device__ __forceinline__ void mfma_tr(f32x16 (&acc)[D / 32], const TrAddr<D>& 
     }
 }
 
-// init + (tile rows 32 mt ..) . (resident rows)^T; roff: row_off() of this lane for mt
+// init + (32 tile rows from `tile` on) . (resident rows)^T; roff: row_off() of this lane
 template <int D>
 __device__ __forceinline__ f32x16 mfma_rows(const char* tile, int roff, const bf16x8 (&b)[D / 16], f32x16 init) {
 #pragma unroll
@@ -171,9 +171,8 @@ __device__ __forceinline__ f32x16 mfma_rows(const char* tile, int roff, const bf
     return init;
 }
 template <int D>
-__device__ __forceinline__ int row_off(int mt, int l31, int hi) {
-    const int r = mt * 32 + l31;
-    return r * 2 * D + ((hi ^ swz<D>(r)) << 4);
+__device__ __forceinline__ int row_off(int l31, int hi) {  // swz() repeats every 16 rows: rows 32 further are 64 D bytes further
+    return l31 * 2 * D + ((hi ^ swz<D>(l31)) << 4);
 }
 
 __device__ __forceinline__ f32x16 splat16(float v) {
@@ -367,8 +366,8 @@ __device__ __forceinline__ bf16x8 pack8(const float* f) {
 
 // The key side of the forward and dQ kernels: K and V tiles through the ring, key masks, and the loop over the tiles.
 // MASK instantiations take every tile through the biased path; the others only a last tile that is not full, behind the
-// loop (one path inside the loop: a second one costs a copy of the accumulators per tile).  LONE: the only tile of a
-// sequence goes there too, and `tile` is told.
+// loop (one path inside the loop: a second one costs a copy of the accumulators per tile).  LONE: there is one tile, and it
+// goes there too.
 template <int D, int KT, bool MASK, bool LONE, typename F>
 __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, const unsigned char* mask, const Span& sp, int kvh,
                                               char* smem, float (*bias)[KT], int wave, int lane, F tile) {
@@ -398,7 +397,7 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
         mb = mask_at(1);
     }
     stage(0, 0, bits);
-    const int nloop = LONE && nt == 1 ? 0 : MASK ? nt : sp.len / KT;
+    const int nloop = LONE ? 0 : MASK ? nt : sp.len / KT;
     for (int kt = 0; kt < nloop; ++kt) {
         const int cur = (kt & 1) * SLOT;
         if constexpr (MASK)
@@ -414,7 +413,7 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
         if (kt + 1 < nt) stage(SLOT - cur, kt + 1, bits);
         if constexpr (MASK)
             if (now == 0) continue;  // every wave has the same bits
-        tile(std::integral_constant<bool, MASK>{}, false, cur, bias[kt & 1]);
+        tile(std::integral_constant<bool, MASK>{}, cur, bias[kt & 1]);
     }
     if ((LONE || !MASK) && nloop < nt) {  // rows past the end landed as zeros
         const int cur = (nloop & 1) * SLOT;
@@ -423,8 +422,69 @@ __device__ __forceinline__ void for_key_tiles(const View& k, const View& v, cons
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if (!MASK || bits != 0) tile(std::true_type{}, LONE && nt == 1, cur, bias[0]);
+        if (!MASK || bits != 0) tile(std::true_type{}, cur, bias[0]);
     }
+}
+
+// A lane's row of its block.  Where it is stored it is worked out anew, from a lane number that no register has kept (own_lane(),
+// which the compiler cannot see to be the same): the loops have none to spare.
+__device__ __forceinline__ int own_lane() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+struct OwnRow {
+    int64_t tok;
+    bool on;
+    __device__ __forceinline__ OwnRow(const Span& sp, int wave, int lane) {
+        const int row = sp.first + wave * 32 + (lane & 31);
+        on = row < sp.len;
+        tok = sp.s0 + (on ? row : sp.len - 1);
+    }
+};
+
+// ---- sequences of few keys -----------------------------------------------------------------------------------------------
+// dS = P (dP - delta) sums to zero over a query's keys, so where few are averaged dq and dk are small differences, and what
+// rounding leaves in dS counts.  Where at most 64 keys of a sequence take part, masked ones not counted, the backward pass
+//   * takes delta + rowsum(P (dP - delta)) for delta, which is free of the rounding of out, and
+//   * puts dS into its products in two bf16 parts.
+// dq of 2, 4 and 16 keys (among 130 tokens) is off by 4.0e-3, 3.0e-3, 2.2e-3 of its norm without the first; of 64 keys by 2.4e-3
+// without the second; with both by 1.7e-3, which is the rounding of dq alone.  Backward pass of 500 sequences of 64 tokens, 18
+// heads: 216 and 234 us.  For sequences of up to 512 keys the second part would make 64 x 512 tokens 354 -> 486 us.
+// The rule looks at the sequence's own keys alone: a padded row's gradients are as exact as the packed sequence's, whatever else
+// is in the call.
+constexpr int AG_FEW_KEYS = 64;
+
+// Masked sequences count 512 keys at a time and stop behind the 64th, so that all but very sparse masks cost one read (64 x 512
+// tokens with a mask, backward pass: 364 and 371 us).
+__device__ __forceinline__ bool few_keys(const unsigned char* mask, const Span& sp, int lane) {
+    if (!mask || sp.len <= AG_FEW_KEYS) return sp.len <= AG_FEW_KEYS;
+    int n = 0;
+    for (int r0 = 0; r0 < sp.len && n <= AG_FEW_KEYS; r0 += 512) {
+        unsigned char m[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = mask_byte(mask, sp.s0, r0 + 64 * i + lane, sp.len);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += __popcll(__ballot(m[i] != 0));
+    }
+    return n <= AG_FEW_KEYS;
+}
+
+// What the rounding of f to `a` leaves, rounded again: f is off by 2^-17 relative at most in the two parts together.
+struct Rest { bf16x8 b[2]; };
+__device__ __forceinline__ Rest rest_of(const float (&f)[16], const bf16x8 (&a)[2]) {
+    float r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = f[i] - (float)a[i >> 3][i & 7];
+    return Rest{{pack8(r), pack8(r + 8)}};
+}
+// acc += X^T . f, f in two parts, both formed before either product and one product at a time: the kernels that call this have
+// no registers to spare.
+template <int D, int MT>
+__device__ __forceinline__ void mfma_tr_two(f32x16 (&acc)[D / 32], const TrAddr<D>& ta, unsigned tile, const float (&f)[16]) {
+    __builtin_amdgcn_sched_barrier(0);
+    const bf16x8 a[2] = {pack8(f), pack8(f + 8)};
+    const Rest rest = rest_of(f, a);
+    __builtin_amdgcn_sched_barrier(0);
+    mfma_tr<D, MT>(acc, ta, tile, a);
+    mfma_tr<D, MT>(acc, ta, tile, rest.b);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -468,7 +528,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 3) void a
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8*)(qp + ks * 16);
     }
-    const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
+    const int koff = row_off<D>(l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
@@ -477,11 +537,11 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 3) void a
     // the range).  That spares the maximum over every tile (1136 -> 933 us at 4 x 4096 with the masks' own kernels).
     float mc = 0.f, l = 0.f;
     bool fresh = true;  // no reference yet
-    for_key_tiles<D, KT, MASK, false>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, bool, int cur, const float* st) {
+    for_key_tiles<D, KT, MASK, false>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, int cur, const float* st) {
         constexpr bool BIASED = decltype(biased)::value;
         f32x16 s[MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt] = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
+        for (int mt = 0; mt < MT; ++mt) s[mt] = mfma_rows<D>(smem + cur + mt * 64 * D, koff, qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
         bf16x8 p[MT][2];
         float ps;
         auto probabilities = [&] {
@@ -534,35 +594,21 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? (MASK ? 3 : 4) : 3) void a
 }
 
 // ---- backward: dQ and delta --------------------------------------------------------------------------------------------
-template <int D, bool MASK>
-__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_kernel(View dout, View q, View k, View v, View o,
-                                                                    const float* __restrict__ lse,
-                                                                    float* __restrict__ delta, OutView dq,
-                                                                    const int* __restrict__ cu, int n_seg,
-                                                                    const unsigned char* __restrict__ mask, int N,
-                                                                    int group, Order od, float scale) {
+// A block's rows, for sequences of many keys, of few in one tile, and of few among masked ones in several tiles: the three share
+// no registers, so that none spills for another.
+enum Keys { MANY, FEW_ONE_TILE, FEW_SCATTERED };
+template <int D, bool MASK, Keys KEYS>
+__device__ __forceinline__ void dq_rows(const View& dout, const View& q, const View& k, const View& v, const View& o,
+                                        const float* __restrict__ lse, float* __restrict__ delta, const OutView& dq,
+                                        const unsigned char* __restrict__ mask, int N, int group, float scale, int head,
+                                        const Span& sp, char* smem, float (*bias)[TR], int wave, int lane) {
     constexpr int TILE = TR * 2 * D;
-    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
-    __shared__ __attribute__((aligned(16))) float bias[2][TR];
-    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int head;
-    Span sp;
-    if (!find_span(od, cu, n_seg, N, head, sp)) return;
-    const int row = sp.first + wave * 32 + l31;
-    const bool on = row < sp.len;
-    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
-    __bf16* op = dq.p + tok * dq.tok + head * dq.head;
-    f32x16 acc[D / 32];
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t) acc[t] = splat16(0.f);
-    if (sp.dead) {
-        store_row<D>(op, acc, 0.f, hi, on);
-        return;
-    }
+    const int l31 = lane & 31, hi = lane >> 5;
     bf16x8 qf[D / 16], gf[D / 16];
-    float dl = 0.f;
+    float dl = 0.f, nl;
     {
+        const int64_t tok = OwnRow(sp, wave, lane).tok;
+        nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;  // +inf only where every tile is skipped
         const __bf16* qp = q.p + tok * q.tok + head * q.head + hi * 8;
         const __bf16* gp = dout.p + tok * dout.tok + head * dout.head + hi * 8;
         const __bf16* xp = o.p + tok * o.tok + head * o.head + hi * 8;
@@ -577,84 +623,125 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
     }
     dl = half_sum(dl);
     const float c = scale * AG_LOG2E;
-    const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;  // +inf only where every tile is skipped
-    const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
+    const int koff = row_off<D>(l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
     f32x16 nd = splat16(-dl);  // dP starts from -delta
 
-    for_key_tiles<D, TR, MASK, true>(k, v, mask, sp, head / group, smem, bias, wave, lane, [&](auto biased, bool lone, int cur, const float* st) {
-        constexpr bool BIASED = decltype(biased)::value;
-        // delta + rowsum(P (dP - delta)) is delta without the rounding of out, which counts where few keys are averaged: dq of
-        // 20 .. 64 tokens is off by 2.4e-3 instead of 2.6e-3 (2.4e-3 is the rounding of dS and dq), of one token by nothing.
-        // For a sequence of one tile it costs two products more and no reads (500 x 64 tokens, backward pass: 232 -> 236 us).
-        if (BIASED && lone) {
-            float more = 0.f;
+    f32x16 acc[D / 32];
+    auto clear = [&] {
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, rows16(st, mt, hi));
-                const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], gf, nd);
+        for (int t = 0; t < D / 32; ++t) acc[t] = splat16(0.f);
+    };
+    auto half = [&](auto mt_, auto biased, int cur, const float* st) {
+        constexpr int mt = decltype(mt_)::value;
+        const f32x16 s = mfma_rows<D>(smem + cur + mt * 64 * D, koff, qf, decltype(biased)::value ? rows16(st, mt, hi) : splat16(0.f));
+        const f32x16 dp = mfma_rows<D>(smem + cur + TILE + mt * 64 * D, koff, gf, nd);
+        float e[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) more += __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
-            }
-            nd = splat16(nd[0] - half_sum(more));
-        }
-        auto half = [&](auto mt_) {
-            constexpr int mt = decltype(mt_)::value;
-            const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], qf, BIASED ? rows16(st, mt, hi) : splat16(0.f));
-            const f32x16 dp = mfma_rows<D>(smem + cur + TILE, koff[mt], gf, nd);
-            float e[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
+        if constexpr (KEYS != MANY) {
+            mfma_tr_two<D, mt>(acc, ta, lds0 + cur, e);
+        } else {
             const bf16x8 ds[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with K
             mfma_tr<D, mt>(acc, ta, lds0 + cur, ds);
-        };
-        half(std::integral_constant<int, 0>{});
-        half(std::integral_constant<int, 1>{});
-    });
-    if (on && hi == 0) delta[(int64_t)head * N + tok] = -nd[0];
-    store_row<D>(op, acc, scale, hi, on);
+        }
+    };
+    auto both = [&](auto biased, int cur, const float* st) {
+        half(std::integral_constant<int, 0>{}, biased, cur, st);
+        half(std::integral_constant<int, 1>{}, biased, cur, st);
+    };
+    auto more = [&](int cur, const float* st) {  // this lane's part of rowsum(P (dP - delta)) over a tile
+        float m = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const f32x16 s = mfma_rows<D>(smem + cur + mt * 64 * D, koff, qf, rows16(st, mt, hi));
+            const f32x16 dp = mfma_rows<D>(smem + cur + TILE + mt * 64 * D, koff, gf, nd);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) m += __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
+        }
+        return m;
+    };
+    auto tiles = [&](auto lone, auto tile) {
+        for_key_tiles<D, TR, MASK, decltype(lone)::value>(k, v, mask, sp, head / group, smem, bias, wave, lane, tile);
+    };
+    clear();
+    if constexpr (KEYS == MANY) {
+        tiles(std::false_type{}, [&](auto biased, int cur, const float* st) { both(biased, cur, st); });
+    } else if constexpr (KEYS == FEW_ONE_TILE) {
+        tiles(std::true_type{}, [&](auto biased, int cur, const float* st) {
+            nd = splat16(nd[0] - half_sum(more(cur, st)));
+            both(biased, cur, st);
+        });
+    } else {  // delta from a pass of its own
+        float m = 0.f;
+        tiles(std::false_type{}, [&](auto, int cur, const float* st) { m += more(cur, st); });
+        nd = splat16(nd[0] - half_sum(m));
+        __syncthreads();  // the ring and the biases have been read
+        clear();
+        tiles(std::false_type{}, [&](auto biased, int cur, const float* st) { both(biased, cur, st); });
+    }
+    const int at = own_lane();
+    const OwnRow r(sp, wave, at);
+    if (r.on && at < 32) delta[(int64_t)head * N + r.tok] = -nd[0];
+    store_row<D>(dq.p + r.tok * dq.tok + head * dq.head, acc, scale, at >> 5, r.on);
+}
+
+template <int D, bool MASK>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_kernel(View dout, View q, View k, View v, View o,
+                                                                    const float* __restrict__ lse,
+                                                                    float* __restrict__ delta, OutView dq,
+                                                                    const int* __restrict__ cu, int n_seg,
+                                                                    const unsigned char* __restrict__ mask, int N,
+                                                                    int group, Order od, float scale) {
+    constexpr int TILE = TR * 2 * D;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];
+    __shared__ __attribute__((aligned(16))) float bias[2][TR];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int head;
+    Span sp;
+    if (!find_span(od, cu, n_seg, N, head, sp)) return;
+    if (sp.dead) {
+        const OwnRow r(sp, wave, lane);
+        f32x16 z[D / 32];
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) z[t] = splat16(0.f);
+        store_row<D>(dq.p + r.tok * dq.tok + head * dq.head, z, 0.f, lane >> 5, r.on);
+        return;
+    }
+    auto rows = [&](auto keys) {
+        dq_rows<D, MASK, decltype(keys)::value>(dout, q, k, v, o, lse, delta, dq, mask, N, group, scale, head, sp, smem, bias, wave, lane);
+    };
+    if (sp.len <= TR) return rows(std::integral_constant<Keys, FEW_ONE_TILE>{});
+    if constexpr (MASK)
+        if (few_keys(mask, sp, lane)) return rows(std::integral_constant<Keys, FEW_SCATTERED>{});
+    rows(std::integral_constant<Keys, MANY>{});
 }
 
 // ---- backward: dK and dV -----------------------------------------------------------------------------------------------
 // At head dim 128 the accumulators take 128 registers and K's fragments 32; V's would leave one wave per SIMD, so they are
 // read from LDS where they are used (LDS reads run at 256 bytes a cycle, a third of the time unused), and the ring holds
 // 32-row tiles: 64 KiB a workgroup, two of them on a CU.
-template <int D>
-__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_kernel(View dout, View q, View k, View v,
-                                                                      const float* __restrict__ lse,
-                                                                      const float* __restrict__ delta, OutView dk,
-                                                                      OutView dv, const int* __restrict__ cu, int n_seg,
-                                                                      const unsigned char* __restrict__ mask, int N,
-                                                                      int group, Order od, float scale) {
+constexpr int dkdv_rt(int D) { return D == 128 ? 32 : 64; }  // rows of a streamed tile
+
+template <int D, bool FEW>
+__device__ __forceinline__ void dkdv_rows(const View& dout, const View& q, const View& k, const View& v,
+                                          const float* __restrict__ lse, const float* __restrict__ delta, const OutView& dk,
+                                          const OutView& dv, int N, int group, float scale, int kvh, const Span& sp, bool live,
+                                          char* smem, float (*stat)[2][dkdv_rt(D)], int wave, int lane) {
     constexpr bool VL = D == 128;
-    constexpr int RT = VL ? 32 : 64, TILE = RT * 2 * D, SLOT = 2 * TILE;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * SLOT + (VL ? AG_BLK * 2 * D : 0)];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][RT];  // slot, (-lse / scale, -delta), row of the tile
-    const int lane = threadIdx.x & 63, l31 = lane & 31, hi = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int kvh;
-    Span sp;
-    if (!find_span(od, cu, n_seg, N, kvh, sp)) return;
-    const int row = sp.first + wave * 32 + l31;
-    const bool on = row < sp.len;
-    const int64_t tok = sp.s0 + (on ? row : sp.len - 1);
-    __bf16* okp = dk.p + tok * dk.tok + kvh * dk.head;
-    __bf16* ovp = dv.p + tok * dv.tok + kvh * dv.head;
+    constexpr int RT = dkdv_rt(D), TILE = RT * 2 * D, SLOT = 2 * TILE;
+    const int l31 = lane & 31, hi = lane >> 5;
     f32x16 ak[D / 32], av[D / 32];
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = splat16(0.f);
-    const bool live = on && !sp.dead && (!mask || mask[tok]);
-    if (!__syncthreads_or(live)) {  // no key of the block takes part
-        store_row<D>(okp, ak, 0.f, hi, on);
-        store_row<D>(ovp, av, 0.f, hi, on);
-        return;
-    }
     // A key that takes no part has its own lane: its column is computed, from zero rows where its fragments are registers,
     // and not used.
     bf16x8 kf[D / 16], vf[VL ? 1 : D / 16];
     {
+        const int64_t tok = OwnRow(sp, wave, lane).tok;
         const __bf16* kp = k.p + tok * k.tok + kvh * k.head + hi * 8;
         const __bf16* vp = v.p + tok * v.tok + kvh * v.head + hi * 8;
 #pragma unroll
@@ -704,8 +791,8 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
         if (++qt == nt) { qt = 0; ++gq; }
     };
     stage(0);
-    const int koff[2] = {row_off<D>(0, l31, hi), row_off<D>(1, l31, hi)};
-    const int voff = 2 * SLOT + wave * 32 * 2 * D + row_off<D>(0, l31, hi);
+    const int koff = row_off<D>(l31, hi);
+    const int voff = 2 * SLOT + wave * 32 * 2 * D + row_off<D>(l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
@@ -713,15 +800,15 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
 
     auto half = [&](auto mt_, int cur, const float* st) {
         constexpr int mt = decltype(mt_)::value;
-        const f32x16 s = mfma_rows<D>(smem + cur, koff[mt], kf, rows16(st, mt, hi));  // Q K^T - lse / scale
+        const f32x16 s = mfma_rows<D>(smem + cur + mt * 64 * D, koff, kf, rows16(st, mt, hi));  // Q K^T - lse / scale
         f32x16 dp = rows16(st + RT, mt, hi);                                          // dO V^T - delta
         if constexpr (VL) {
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(smem + cur + TILE + (koff[mt] ^ (ks << 5))),
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(smem + cur + TILE + mt * 64 * D + (koff ^ (ks << 5))),
                                                              *(const bf16x8*)(smem + (voff ^ (ks << 5))), dp, 0, 0, 0);
         } else {
-            dp = mfma_rows<D>(smem + cur + TILE, koff[mt], vf, dp);
+            dp = mfma_rows<D>(smem + cur + TILE + mt * 64 * D, koff, vf, dp);
         }
         float e[16], f[16];
 #pragma unroll
@@ -730,9 +817,15 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
             f[r] = e[r] * dp[r];
         }
         // 2^-8 relative at most, for the products with dO and Q
-        const bf16x8 p[2] = {pack8(e), pack8(e + 8)}, ds[2] = {pack8(f), pack8(f + 8)};
-        mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
-        mfma_tr<D, mt>(ak, ta, lds0 + cur, ds);
+        const bf16x8 p[2] = {pack8(e), pack8(e + 8)};
+        if constexpr (FEW) {
+            mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
+            mfma_tr_two<D, mt>(ak, ta, lds0 + cur, f);
+        } else {
+            const bf16x8 ds[2] = {pack8(f), pack8(f + 8)};
+            mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
+            mfma_tr<D, mt>(ak, ta, lds0 + cur, ds);
+        }
     };
     for (int i = 0; i < total; ++i) {
         const int cur = (i & 1) * SLOT;
@@ -748,8 +841,40 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
 #pragma unroll
         for (int t = 0; t < D / 32; ++t) ak[t] = av[t] = splat16(0.f);
     }
-    store_row<D>(okp, ak, scale, hi, on);
-    store_row<D>(ovp, av, 1.f, hi, on);
+    const int at = own_lane();
+    const OwnRow r(sp, wave, at);
+    store_row<D>(dk.p + r.tok * dk.tok + kvh * dk.head, ak, scale, at >> 5, r.on);
+    store_row<D>(dv.p + r.tok * dv.tok + kvh * dv.head, av, 1.f, at >> 5, r.on);
+}
+
+template <int D>
+__global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_kernel(View dout, View q, View k, View v,
+                                                                      const float* __restrict__ lse,
+                                                                      const float* __restrict__ delta, OutView dk,
+                                                                      OutView dv, const int* __restrict__ cu, int n_seg,
+                                                                      const unsigned char* __restrict__ mask, int N,
+                                                                      int group, Order od, float scale) {
+    constexpr int RT = dkdv_rt(D);
+    __shared__ __attribute__((aligned(1024))) char smem[4 * RT * 2 * D + (D == 128 ? AG_BLK * 2 * D : 0)];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][RT];  // slot, (-lse / scale, -delta), row of the tile
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int kvh;
+    Span sp;
+    if (!find_span(od, cu, n_seg, N, kvh, sp)) return;
+    const OwnRow r(sp, wave, lane);
+    const bool live = r.on && !sp.dead && (!mask || mask[r.tok]);
+    const bool few = few_keys(mask, sp, lane);
+    if (!__syncthreads_or(live)) {  // no key of the block takes part
+        f32x16 z[D / 32];
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) z[t] = splat16(0.f);
+        store_row<D>(dk.p + r.tok * dk.tok + kvh * dk.head, z, 0.f, lane >> 5, r.on);
+        store_row<D>(dv.p + r.tok * dv.tok + kvh * dv.head, z, 0.f, lane >> 5, r.on);
+        return;
+    }
+    if (few) dkdv_rows<D, true>(dout, q, k, v, lse, delta, dk, dv, N, group, scale, kvh, sp, live, smem, stat, wave, lane);
+    else dkdv_rows<D, false>(dout, q, k, v, lse, delta, dk, dv, N, group, scale, kvh, sp, live, smem, stat, wave, lane);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------
@@ -786,22 +911,6 @@ __device__ __forceinline__ void join_rows(float* area, const f32x16 (&acc)[D / 3
         if (row < rows)
             *(u32x4*)(p + row * tok + col + j) = u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
     }
-}
-
-// acc += X^T . f, f rounded to bf16, and in sequences of up to 512 tokens the rest of f as well, rounded again.  dS sums to zero
-// over a row, so that dq and dk lose most to its rounding where few terms are added, and there the second product is cheap: 21 to
-// 64 tokens are off by 1.7e-3 instead of 2.4e-3, which is the rounding of dq and dk alone, 8 x 512 by 1.8e-3 instead of 2.5e-3
-// (backward pass, 2 heads: 31.3 and 32.3 us); at one of 4096, 4 heads, it would be 103 and 119 us.
-template <int D>
-__device__ __forceinline__ void mfma_tr_rest(f32x16 (&acc)[D / 32], const TrAddr<D>& ta, unsigned tile, const float (&f)[16], int len) {
-    const bf16x8 a[2] = {pack8(f), pack8(f + 8)};
-    mfma_tr<D, 0>(acc, ta, tile, a);
-    if (len > 512) return;  // uniform
-    float rest[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) rest[r] = f[r] - (float)a[r >> 3][r & 7];
-    const bf16x8 b[2] = {pack8(rest), pack8(rest + 8)};
-    mfma_tr<D, 0>(acc, ta, tile, b);
 }
 
 // Tiles wave, wave + 4, ... of 32 keys, through the wave's own ring (2 slots of K and V).
@@ -870,7 +979,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_fwd_few_k
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const bf16x8*)(qp + ks * 16);
     }
-    const int koff = row_off<D>(0, l31, hi);
+    const int koff = row_off<D>(l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     char* ring = smem + wave * RING;
@@ -966,7 +1075,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dq_fe
     f32x16 nd = splat16(-half_sum(dl));
     const float c = scale * AG_LOG2E;
     const float nl = -lse[(int64_t)head * N + tok] * AG_LOG2E;
-    const int koff = row_off<D>(0, l31, hi);
+    const int koff = row_off<D>(l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     char* ring = smem + wave * RING;
@@ -978,7 +1087,8 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dq_fe
 #pragma unroll
         for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
     };
-    if (sp.len <= TR) {  // delta without the rounding of out, as in the large kernel
+    const bool few = few_keys(mask, sp, lane);
+    if (few) {  // delta without the rounding of out, as in the large kernel
         float more = 0.f;
         for_own_tiles<D>(k, v, mask, sp, head / group, ring, bias[wave], wave, lane, [&](int cur, const float* st) {
             products(cur, st);
@@ -996,7 +1106,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dq_fe
     if (wave == 0 && on && hi == 0) delta[(int64_t)head * N + tok] = -nd[0];
     for_own_tiles<D>(k, v, mask, sp, head / group, ring, bias[wave], wave, lane, [&](int cur, const float* st) {
         products(cur, st);
-        mfma_tr_rest<D>(acc, ta, lds0 + cur, e, sp.len);
+        const bf16x8 ds[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with K
+        mfma_tr<D, 0>(acc, ta, lds0 + cur, ds);
+        if (few) mfma_tr<D, 0>(acc, ta, lds0 + cur, rest_of(e, ds).b);
     });
     __syncthreads();
     join_rows<D>((float*)smem, acc, scale, wave, lane, dq.p + (sp.s0 + sp.first) * dq.tok + head * dq.head, dq.tok, sp.len - sp.first);
@@ -1067,12 +1179,13 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dkdv_
         next = hi ? -x : -x * inv_scale;
         qt += AG_WAVES;
     };
-    const int koff = row_off<D>(0, l31, hi);
+    const int koff = row_off<D>(l31, hi);
     TrAddr<D> ta;
     ta.init(lane);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(ring);
     const float c = scale * AG_LOG2E;
     if (wave < total) stage(0);
+    const bool few = few_keys(mask, sp, lane);
     for (int i = wave, j = 0; i < total; i += AG_WAVES, j ^= 1) {
         const int cur = j * SLOT;
         stat[wave][j][hi][l31] = next;
@@ -1089,7 +1202,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dkdv_
         }
         const bf16x8 p[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with dO
         mfma_tr<D, 0>(av, ta, lds0 + cur + TILE, p);
-        mfma_tr_rest<D>(ak, ta, lds0 + cur, f, sp.len);
+        const bf16x8 ds[2] = {pack8(f), pack8(f + 8)};  // the same, for the product with Q
+        mfma_tr<D, 0>(ak, ta, lds0 + cur, ds);
+        if (few) mfma_tr<D, 0>(ak, ta, lds0 + cur, rest_of(f, ds).b);
     }
     if (!live) {
 #pragma unroll

@@ -218,8 +218,10 @@ def attention_varlen_forward(q, k, v, cu_seqlens, scale: float | None = None, ke
 def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float | None = None, key_mask=None):
     """Gradients of `attention_varlen_forward` -> (dq, dk, dv), dense bf16 in the shapes of q, k and v.  out and lse are the
     forward call's, on the same inputs.  Probabilities and their gradients are rounded to bf16 for the products with q, k and
-    dout (the gradients in two parts where that costs next to nothing: few and short sequences); every sum is fp32, and shared
-    key heads sum over their query heads in fp32."""
+    dout; every sum is fp32, and shared key heads sum over their query heads in fp32.  Sequences of at most 64 unmasked keys
+    lose nothing of dq and dk but the rounding of the results: delta is summed without the rounding of out, and the gradients of
+    the probabilities enter in two bf16 parts.  That depends on a sequence's own keys, not on padding or on the rest of the
+    call."""
     gpu, N, H, G, D = _check_attention(q, k, v, cu_seqlens, key_mask)
     scale = _scale(scale, D)
     _need(dout, "dout", _BF16, gpu)

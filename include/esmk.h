@@ -277,8 +277,9 @@ int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v, void* out,
                          int n_kv_heads, int head_dim, float scale, esmk_stream_t stream);
 /* Gradients of the same with respect to q, k and v, from out and lse of esmk_attn_varlen_fwd on the same inputs.  strides:
  * 16 values for dout, q, k, v, out, dq, dk, dv.  dk and dv are summed over the query heads that share a key head.  Masked
- * keys, queries without a key and tokens in no sequence get zeros.  workspace: esmk_attn_varlen_bwd_workspace_bytes, owned by
- * this call while it runs. */
+ * keys, queries without a key and tokens in no sequence get zeros.  Probabilities and their gradients are rounded to bf16 for
+ * the second products; in sequences of at most 64 unmasked keys the gradients enter in two parts, and rowsum(dout out) is summed
+ * again without the rounding of out.  workspace: esmk_attn_varlen_bwd_workspace_bytes, owned by this call while it runs. */
 size_t esmk_attn_varlen_bwd_workspace_bytes(int n_tokens, int n_heads);
 int esmk_attn_varlen_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                          void* dq, void* dk, void* dv, const int64_t* strides, const int32_t* cu_seqlens, int n_segments,

@@ -434,6 +434,63 @@ def test_attention_padded_batch_equals_packed():
     assert torch.equal(got[0][at], want[0]) and not got[3][~mask].any()
 
 
+def few_key_buffers(at, N, q, k, v, dout, g):
+    """The packed tokens at the places `at` of a buffer of N tokens that holds anything elsewhere, with the mask of
+    those places; dout is zero elsewhere."""
+    wide = lambda t: randn(g, N, *t.shape[1:]).bfloat16().index_copy(0, at, t.contiguous())
+    mask = torch.zeros(N, dtype=torch.bool, device="cuda").index_fill(0, at, True)
+    return wide(q), wide(k), wide(v), wide(dout) * mask[:, None, None], mask
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scattered", [False, True])
+@pytest.mark.parametrize("L", [70, 130, 600, 1100])
+def test_attention_few_live_keys_among_padding(L, scattered, D):
+    """Sequences of 1 to 64 live keys, padded at their end or scattered among masked tokens: the bounds of the packed
+    sequences, whose delta is free of out's rounding and whose dS has two parts.  The sums have the same terms; masked keys add
+    zeros.  In few blocks and in many."""
+    lens = [1, 2, 3, 5, 17, 33, 64]
+    q, k, v, cu, cut, dout, g = attention_inputs(60 + L + D, lens, 4, 2, D)
+    at = []
+    for i, n in enumerate(lens):
+        where = torch.randperm(L, generator=torch.Generator().manual_seed(i))[:n].sort()[0] if scattered else torch.arange(n)
+        at.append(where + i * L)
+    at = torch.cat(at).cuda()
+    want, tol = attention_oracle(q, k, v, cu, D ** -0.5, None, dout, short=True, rest=True)
+    wq, wk, wv, wd, mask = few_key_buffers(at, len(lens) * L, q, k, v, dout, g)
+    wcu = torch.arange(len(lens) + 1, dtype=torch.int32, device="cuda") * L
+    for r in (1, copies(len(mask), len(lens), 2)):
+        many = lambda t: t.repeat(1, r, 1)
+        got = attention_all(many(wq), many(wk), many(wv), wcu, many(wd), mask=mask)
+        for a, b, t, n in zip(got[2:], want[2:], tol[2:], ("dq", "dk", "dv")):
+            a = a.view(len(mask), r, -1, D).transpose(0, 1)
+            within(a[:, at], b.expand_as(a[:, at]), t, f"{n}, {r} copies")
+            assert n == "dq" or not a[:, ~mask].any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_gradients_of_few_keys_do_not_depend_on_the_rest_of_the_call(D, masked):
+    """The same short sequences alone, among long ones, and with more heads: dS in two parts in all of them."""
+    short = [1, 5, 64, 2, 33, 40, 63, 3]
+    q, k, v, cu, cut, dout, g = attention_inputs(80 + D, short + [900, 70, 1300], 4, 2, D)
+    n = sum(short)
+    mask = None
+    if masked:
+        mask = torch.rand(len(q), generator=g, device="cuda") > 0.3
+        mask[cu[2]:cu[3]:2] = True
+    want, tol = attention_oracle(q[:n], k[:n], v[:n], cu[:len(short) + 1], D ** -0.5, None if mask is None else mask[:n], dout[:n],
+                                 short=True, rest=True)
+    alone = (q[:n], k[:n], v[:n], cut[:len(short) + 1], dout[:n], None if mask is None else mask[:n])
+    r = copies(len(q), len(cu) - 1, 2)
+    many = lambda t: t.repeat(1, r, 1)
+    for args in (alone, (q, k, v, cut, dout, mask), (many(q), many(k), many(v), cut, many(dout), mask)):
+        got = attention_all(*args[:5], mask=args[5])
+        for a, b, t, name in zip(got[2:], want[2:], tol[2:], ("dq", "dk", "dv")):
+            a = a[:n].view(n, -1, b.shape[1], D).transpose(0, 1)
+            within(a, b.expand_as(a), t, f"{name}, {len(args[0])} tokens, {args[0].shape[1]} heads")
+
+
 def test_attention_rising_and_falling_scores():
     """Keys whose scores rise from tile to tile by far more than the reference point may lag, and fall again; large values."""
     N = 64 * 9
