@@ -5,7 +5,7 @@
 #include <stdarg.h>
 #include <string.h>
 
-#include "build_id.h"
+#include "esmk_build_id.h"
 #include "common.hpp"
 
 static thread_local char g_err[512] = "";

@@ -50,7 +50,7 @@ typedef void* esmk_stream_t; /* hipStream_t */
 
 int esmk_version(void);
 const char* esmk_last_error(void);
-/* 12 hex digits: hash of the sources this binary was built from (written by the Makefile).  bench.py and the
+/* 12 hex digits: hash of the sources and compiler flags this binary was built from (written by the Makefile).  bench.py and the
  * profiles under profiles/ carry it, so a measured number can be tied to one binary.  No reference counterpart. */
 const char* esmk_build_id(void);
 
