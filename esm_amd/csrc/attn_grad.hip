@@ -724,6 +724,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
 // At head dim 128 the accumulators take 128 registers and K's fragments 32; V's would leave one wave per SIMD, so they are
 // read from LDS where they are used (LDS reads run at 256 bytes a cycle, a third of the time unused), and the ring holds
 // 32-row tiles: 64 KiB a workgroup, two of them on a CU.
+// Both head dims run at their register limit.  The loops over full tiles use no scratch (the lane's row is worked out again at the
+// store, and the path of few keys is a body of its own); a few registers are kept in it around them, and about nine in the loop of
+// few keys (500 x 64 tokens, 18 heads, backward pass 234 us; with twice as many of them 365).
 constexpr int dkdv_rt(int D) { return D == 128 ? 32 : 64; }  // rows of a streamed tile
 
 template <int D, bool FEW>

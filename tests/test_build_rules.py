@@ -13,6 +13,7 @@ COMPILER = """#!/bin/sh
 echo "$*" >> "$NOTES"
 while [ $# -gt 0 ]; do if [ "$1" = -o ]; then out=$2; fi; shift; done
 : > "$out"
+[ -z "$REMARK" ] || echo "$REMARK" >&2
 """
 
 
@@ -29,11 +30,12 @@ def tree(tmp_path):
     cc.write_text(COMPILER)
     cc.chmod(0o755)
 
-    def make(*args):
-        """Sources compiled by one call of make, in any order."""
+    def make(*args, remark=""):
+        """Sources compiled by one call of make, sorted.  remark: what the compiler says."""
         notes = tmp_path / "notes"
         notes.write_text("")
-        subprocess.run(["make", "-C", str(csrc), f"HIPCC={cc}", *args], check=True, capture_output=True, env={**os.environ, "NOTES": str(notes)})
+        subprocess.run(["make", "-C", str(csrc), f"HIPCC={cc}", *args], check=True, capture_output=True,
+                       env={**os.environ, "NOTES": str(notes), "REMARK": remark})
         return sorted(re.findall(r"-c (\S+\.hip)", notes.read_text()))
 
     def build_id(out="obj"):
@@ -82,3 +84,16 @@ def test_a_changed_source_rebuilds_itself_and_the_build_id(tree):
     change(csrc / "pref_loss.hip", "namespace {\n", "namespace {  // changed\n")
     os.utime(csrc / "pref_loss.hip", (2 ** 31, 2 ** 31))
     assert make()[:1] == ["pref_loss.hip"] and build_id() != first
+
+
+@pytest.mark.parametrize("kind,source,most", [((), "attn_grad", 56), (("EXPERIMENTS=1",), "gemm4w", 0), (("EXPERIMENTS=1",), "gemm4v", 0)])
+def test_scratch_beyond_what_is_stated_ends_the_build(tree, kind, source, most):
+    csrc, make, _ = tree
+    said = "k.hip:1:1: remark:     ScratchSize [bytes/lane]: %d [-Rpass-analysis=kernel-resource-usage]"
+    out = csrc / ("xobj" if kind else "obj") / f"{source}.o"
+    target = str(out.relative_to(csrc))
+    with pytest.raises(subprocess.CalledProcessError):
+        make(target, *kind, remark=said % (most + 1))
+    assert not out.exists()
+    make(target, *kind, remark=said % most)
+    assert out.exists()
