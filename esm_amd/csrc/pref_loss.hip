@@ -6,9 +6,9 @@
 //   dL/dz_t = c_t (onehot(y_t) - softmax z_t),  c_t = dL/dl of its sequence, 0 where the token is not scored
 //
 // A token's softmax needs its row of logits alone, a row's gradient needs both sequences of its pair: so one pass over the
-// logits leaves (max, log-sum, log-probability) of every token, a workgroup per pair adds the log-probabilities (in 64
-// bits: a margin is a small difference of two long sums) and leaves c_t, and the backward pass reads the logits once more
-// and writes the gradient.  Sums run in a fixed order.  The first and the last pass are bound by memory (10 ragged pairs over
+// logits leaves (max, sum of exponentials, target's logit) of every token, a workgroup per pair forms the log-probabilities and
+// adds them (in 64 bits: a margin is a small difference of two long sums) and leaves c_t, and the backward pass reads the logits
+// once more and writes the gradient.  Sums run in a fixed order.  The first and the last pass are bound by memory (10 ragged pairs over
 // 4096 bf16 entries: 20 us, 5.0 TB/s, and 31 us, 6.3 TB/s with the logits partly in the cache), the pairs by a few dependent
 // reads (5 to 6 us).
 #include <type_traits>
@@ -17,8 +17,9 @@
 
 namespace {
 
-// token state: max, log of the sum of exp(z - max), log-probability of the target, c_t (until the pair is known: 1 if the
-// token is scored, else 0)
+// token state: max, sum of exp(z - max), the target's logit, c_t (until the pair is known: 1 if the token is scored, else 0).
+// Its log-probability is formed from them in 64 bits (pref_pair_kernel()): one of -5 is off by 2^-22 in 32, and a margin adds up a
+// thousand of those.
 typedef f32x4 TokState;
 
 template <typename T> struct PlT;
@@ -46,14 +47,19 @@ __device__ __forceinline__ void pl_store(__bf16* p, const float (&f)[8]) {
 }
 
 constexpr float PL_LOG2E = 1.4426950408889634f, PL_LN2 = 0.6931471805599453f;
+constexpr float PL_LOG2E_LOW = 1.9259629911e-8f;  // log2(e) - fp32(log2(e))
 
 // exp(x) for x <= 0 with the product x log2(e) carried in two parts: exp2 alone would lose |x| 2^-24 of the result
 __device__ __forceinline__ float pl_exp(float x) {
     const float h = x * PL_LOG2E;
-    const float l = fmaf(x, PL_LOG2E, -h) + x * 1.9259629911e-8f;  // log2(e) - fp32(log2(e))
+    const float l = fmaf(x, PL_LOG2E, -h) + x * PL_LOG2E_LOW;
     const float r = __builtin_amdgcn_exp2f(h);
     return h < -3e38f ? 0.f : fmaf(r * PL_LN2, l, r);  // x = -inf makes l NaN; a NaN x stays one
 }
+// exp(x) as a term of a long sum: x log2(e) rounded once, which is off to either side.  The product with fp32(log2(e)) is off to one
+// side, by 7e-8 of the sum at x = -5, and a margin adds up a thousand tokens' of it: gradients of 10 ragged pairs over 4096 fp32
+// entries off by 1.7e-6, and by 1e-7 so (forward pass of the bf16 ones 21.9 and 23.4 us; with both parts of pl_exp() 27.6).
+__device__ __forceinline__ float pl_exp_term(float x) { return __builtin_amdgcn_exp2f(fmaf(x, PL_LOG2E, x * PL_LOG2E_LOW)); }
 
 // Rows start at any element: a row is covered by 16-byte pieces of memory; the first and the last may hold elements of
 // the neighbouring rows, and are read and written element by element.
@@ -145,16 +151,14 @@ __global__ __launch_bounds__(256) void pref_token_kernel(const T* __restrict__ z
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((f[i][e] - base) * PL_LOG2E);
-        l = l * __builtin_amdgcn_exp2f((m - base) * PL_LOG2E) + s;
+            for (int e = 0; e < E; ++e) s += pl_exp_term(f[i][e] - base);
+        l = fmaf(l, pl_exp(m - base), s);
         m = t;
     }
     const float top = row_max<LPR>(m);
-    l = row_add<LPR>(l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * PL_LOG2E)));
-    if (sub == 0) {
-        const float ls = logf(l);  // no finite logit: log 0, and the row's loss is not finite, as the formula has it
-        tok[row] = TokState{top, ls, (pl_get(z + row * V + y) - top) - ls, 1.f};
-    }
+    l = row_add<LPR>(l * (m == -INFINITY ? 0.f : pl_exp(m - top)));
+    // no finite logit: log 0, and the row's loss is not finite, as the formula has it
+    if (sub == 0) tok[row] = TokState{top, l, pl_get(z + row * V + y), 1.f};
 }
 
 // One workgroup per pair: a few dependent reads long, so a thread requests up to four tokens of both sequences at once.
@@ -174,20 +178,21 @@ __global__ __launch_bounds__(PL_PAIR) void pref_pair_kernel(TokState* __restrict
     double a[2] = {0.0, 0.0};
     int n = 0;
     for (int t0 = threadIdx.x; at[0] + t0 < at[1] || at[1] + t0 < at[2]; t0 += PL_PAIR * AHEAD) {
-        f32x2 v[2][AHEAD];
+        f32x4 v[2][AHEAD];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int t = at[s] + t0 + j * PL_PAIR;
-                v[s][j] = t < at[s + 1] ? *((const f32x2*)(tok + t) + 1) : f32x2{0.f, 0.f};
+                v[s][j] = t < at[s + 1] ? tok[t] : f32x4{0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                a[s] += (double)v[s][j][0];  // 0 where the token is not scored
-                if (s == 0) n += v[s][j][1] != 0.f;
+                if (v[s][j][3] == 0.f) continue;  // not scored
+                a[s] += ((double)v[s][j][2] - (double)v[s][j][0]) - log((double)v[s][j][1]);
+                if (s == 0) ++n;
             }
     }
 #pragma unroll
@@ -258,7 +263,7 @@ __global__ __launch_bounds__(256) void pref_grad_kernel(const T* __restrict__ z,
     const TokState st = tok[row];
     const int64_t y = targets[row];
     const bool on = st[3] != 0.f;  // 0: not scored, or behind the last sequence
-    const float c = on ? (grad ? st[3] * *grad : st[3]) : 0.f;
+    const float c = on ? (grad ? st[3] * *grad : st[3]) : 0.f, minus = -c / st[1];
     const Row<T> r(z, row, V);
     T* out = dz + row * V - r.lead;
     for (int p = sub; p < r.n_pieces; p += LPR) {
@@ -267,10 +272,7 @@ __global__ __launch_bounds__(256) void pref_grad_kernel(const T* __restrict__ z,
         if (on) {
             r.load(p, f, 0.f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float q = pl_exp((f[e] - st[0]) - st[1]);
-                o[e] = c * ((col + e == (int)y ? 1.f : 0.f) - q);
-            }
+            for (int e = 0; e < E; ++e) o[e] = fmaf(pl_exp(f[e] - st[0]), minus, col + e == (int)y ? c : 0.f);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = 0.f;

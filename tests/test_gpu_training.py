@@ -641,6 +641,35 @@ def test_preference_long_sequences_many_pairs_and_a_lead(lens):
     assert not dz[:11].any() and not dz[cu[-1]:].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [60, 1024])
+def test_preference_margin_of_a_long_sequence_has_no_bias(V, dtype):
+    """A margin of 40000 tokens: errors that go either way add up to the root of their number, a bias to all of it.  A token's
+    log-probability takes some dozens of roundings of at most u each: below 8 u in root mean square, and six standard deviations
+    of 40000 of them are asked.  One logit above the others by log V: half of the sum lies that far below the maximum."""
+    n = 40000
+    g = gen(V)
+    z = 0.3 * randn(g, n, V)
+    z[:, V // 3] += math.log(V)
+    z = z.to(dtype)
+    y = torch.randint(0, V, (n,), generator=g, device="cuda")
+    want = torch.log_softmax(z.double(), -1).gather(1, y[:, None]).sum()
+    cut = torch.tensor([0, n, n], dtype=torch.int32, device="cuda")
+    ref = torch.stack([want, torch.zeros_like(want)]).float()  # a margin near zero: the loss shows its error
+    loss, logps, saved = T().preference_loss_forward(z, y, cut, ref, beta=1.0)
+    m = want - ref[0].double()
+    error = 6 * 8 * U * n ** 0.5
+    exact = torch.nn.functional.softplus(-m)
+    assert abs(loss.double() - exact) <= error * torch.sigmoid(-m) + U * exact
+    dz = T().preference_loss_backward(z, y, saved)
+    c = -torch.sigmoid(-m)
+    p = torch.log_softmax(z.double(), -1).exp()
+    grad = c * (torch.nn.functional.one_hot(y, V) - p)
+    # the coefficient is off by the margin's error times sigmoid(m); a probability has a few roundings of its own
+    tol = (error * torch.sigmoid(m) + 4 * U) * grad.abs() + 16 * U * c.abs() * p
+    within(dz, grad, tol * (1 + R[dtype]) + R[dtype] * grad.abs(), "dz")
+
+
 def test_preference_more_than_2_31_elements():
     """Logits and gradients past 2^32 bytes: the last pair against the same pair alone (half the weight among two pairs)."""
     z1, y1, cu, cut, ref, _ = preference_inputs(19, [300, 211], 4096, torch.bfloat16)
