@@ -54,11 +54,23 @@ def _call(gpu, name, *args):
 
 
 def _rows(t, d):
-    """t [..., d] -> (t with dense equally spaced rows, distance of its rows); copies only where no such view exists."""
+    """t [..., d] -> (t with dense equally spaced rows, distance of its rows); copies only where the rows are not dense or do not
+    lie at one distance.  Slices [..., :d] of wider activations do, whatever their number of dimensions."""
     if t.is_contiguous():
         return t, d
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= d:
-        return t, t.stride(0)
+    if t.stride(-1) == 1:
+        ld = after = None  # distance of the rows, and what the next dimension's stride has to be
+        for n, stride in zip(t.shape[-2::-1], t.stride()[-2::-1]):
+            if n == 1:
+                continue
+            if ld is None:
+                ld = stride
+            elif stride != after:
+                break
+            after = stride * n
+        else:
+            if ld is not None and ld >= d:
+                return t, ld
     return t.contiguous(), d
 
 

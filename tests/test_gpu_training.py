@@ -112,6 +112,27 @@ def test_layer_norm_strides_ranks_and_parameter_types():
     assert torch.equal(T().layer_norm_forward(x1, w.bfloat16())[0], T().layer_norm_forward(x1, w.bfloat16().float())[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 192, 1152])
+def test_layer_norm_slices_of_wider_activations(d, dtype):
+    """x and dy as slices of [B, L, 3 d] activations, read in place: the bits of the 2-D slices, and of copies."""
+    g = gen(d)
+    qkv, grads = randn(g, 3, 41, 3 * d).to(dtype), randn(g, 3, 41, 2 * d).to(dtype)
+    w, b = 1 + 0.1 * randn(g, d), 0.1 * randn(g, d)
+    for x, dy in ((qkv[..., :d], grads[..., d:]), (qkv[..., 2 * d:], grads[..., :d]), (qkv[:, :1, d:2 * d], grads[:, 3:4, :d]),
+                  (qkv[:, :40, :d], grads[:, 1:, d:])):
+        got = T().layer_norm_forward(x, w, b)
+        got += T().layer_norm_backward(dy, x, w, got[1])
+        xc, dc = x.reshape(-1, d).contiguous(), dy.reshape(-1, d).contiguous()
+        want = T().layer_norm_forward(xc, w, b)
+        want += T().layer_norm_backward(dc, xc, w, want[1])
+        for p, q in zip(got, want):
+            assert torch.equal(p.reshape(q.shape), q)
+        leaf = x.detach().requires_grad_()
+        T().layer_norm(leaf, w, b).backward(dy)
+        assert torch.equal(leaf.grad.reshape(-1, d), want[2])
+
+
 def test_layer_norm_no_rows_gives_zero_parameter_gradients():
     x, w = torch.empty(0, 96, device="cuda"), torch.ones(96, device="cuda")
     y, st = T().layer_norm_forward(x, w)

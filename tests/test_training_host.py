@@ -112,3 +112,23 @@ def test_host_tensors_are_refused():
         T.layer_norm(x.half(), w)
     with pytest.raises(TypeError):
         T.attention_varlen("q", q, q, cu)
+
+
+def test_rows_of_wider_tensors_are_read_in_place():
+    """`_rows` copies only where the rows do not lie at one distance."""
+    at = lambda t: (t.data_ptr(), t.shape)
+    wide = torch.zeros(2, 5, 3, 4 * 8)
+    qkv = torch.zeros(3, 7, 3 * 16)
+    for t, ld in ((qkv[..., :16], 48), (qkv[..., 16:32], 48), (qkv[:, :1, :16], 7 * 48), (qkv[1:2, :, 32:], 48), (qkv[0, :, 5:21], 48),
+                  (qkv[::2, :1, :16], 14 * 48), (qkv[:, ::7, 1:17], 7 * 48), (wide[..., 3:9], 32), (wide[:, :, 1, :8], 96), (wide[1, :, 2:, :8], 96),
+                  (wide[:, None, :, :, 8:16], 32), (qkv[0, :, :1], 48), (qkv, 48), (qkv[0, 0], 48), (qkv[:0], 48)):
+        rows, got = T._rows(t, t.shape[-1])
+        assert at(rows) == at(t) and got == ld
+        if t.numel():  # row r starts r * ld elements behind the first
+            firsts = [rows.storage_offset() + sum(i * s for i, s in zip(index, rows.stride())) for index in torch.cartesian_prod(
+                *[torch.arange(n) for n in t.shape[:-1]], torch.arange(1)).tolist()] if t.dim() > 1 else [rows.storage_offset()]
+            assert [f - firsts[0] for f in firsts] == [r * ld for r in range(len(firsts))]
+    for t in (qkv[:, :4, :16], wide[:, :, :2, :8], qkv[..., ::3], qkv.transpose(0, 1)[..., :16], qkv[:, :, :16].transpose(1, 2),
+              qkv[:1, :, :16].expand(3, 7, 16), qkv[0, :1, :16].expand(7, 16), torch.zeros(40).as_strided((5, 8), (4, 1))):
+        rows, got = T._rows(t, t.shape[-1])
+        assert rows.is_contiguous() and rows.data_ptr() != t.data_ptr() and got == t.shape[-1] and torch.equal(rows, t)
