@@ -1293,9 +1293,10 @@ extern "C" int esmk_attn_varlen_bwd(const void* dout, const void* q, const void*
                                     size_t workspace_bytes, esmk_stream_t stream) {
     if (int rc = ag_check("esmk_attn_varlen_bwd", cu_seqlens, n_segments, n_tokens, n_heads, n_kv_heads, head_dim, scale)) return rc;
     if (n_tokens == 0) return ESMK_OK;
-    if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv || !strides) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_bwd: null pointer");
+    if (!dout || !q || !k || !v || !out || !lse || !dq || !strides) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_bwd: null pointer");
+    if (!dk != !dv) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_bwd: null pointer (dk and dv are wanted together or not at all)");
     const void* ps[8] = {dout, q, k, v, out, dq, dk, dv};
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < (dk ? 8 : 6); ++i)
         if (!ag_strides(ps[i], strides + 2 * i, head_dim))
             ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_attn_varlen_bwd: tensor %d: address and strides must be multiples of 16 bytes, token stride >= head_dim", i);
     if (!workspace || workspace_bytes < esmk_attn_varlen_bwd_workspace_bytes(n_tokens, n_heads) || ((uintptr_t)workspace & 3))
@@ -1313,10 +1314,12 @@ extern "C" int esmk_attn_varlen_bwd(const void* dout, const void* q, const void*
                               : (key_mask ? attn_bwd_dq_kernel<128, true> : attn_bwd_dq_kernel<128, false>);
     hipLaunchKernelGGL(kq, dim3(oq.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), in(4), lse, delta, ov(5),
                        cu_seqlens, n_segments, key_mask, n_tokens, group, oq, scale);
-    auto* kk = few_k ? (head_dim == 64 ? attn_bwd_dkdv_few_kernel<64> : attn_bwd_dkdv_few_kernel<128>)
-                     : (head_dim == 64 ? attn_bwd_dkdv_kernel<64> : attn_bwd_dkdv_kernel<128>);
-    hipLaunchKernelGGL(kk, dim3(ok.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), lse, delta, ov(6), ov(7),
-                       cu_seqlens, n_segments, key_mask, n_tokens, group, ok, scale);
+    if (dk) {
+        auto* kk = few_k ? (head_dim == 64 ? attn_bwd_dkdv_few_kernel<64> : attn_bwd_dkdv_few_kernel<128>)
+                         : (head_dim == 64 ? attn_bwd_dkdv_kernel<64> : attn_bwd_dkdv_kernel<128>);
+        hipLaunchKernelGGL(kk, dim3(ok.grid), dim3(AG_WAVES * 64), 0, s, in(0), in(1), in(2), in(3), lse, delta, ov(6), ov(7),
+                           cu_seqlens, n_segments, key_mask, n_tokens, group, ok, scale);
+    }
     ESMK_CHECK_LAUNCH("esmk_attn_varlen_bwd");
     return ESMK_OK;
 }

@@ -279,7 +279,7 @@ __global__ __launch_bounds__(ng_threads(WPR)) void norm_bwd_kernel(const T* __re
         row_sum2<WPR>(c1, c2, buf, half);
         c1 *= inv_d;
         c2 *= inv_d;
-        const __amdgpu_buffer_rsrc_t dr = ng_row(dx + (int64_t)(row < M ? row : 0) * d, row < M ? bytes : 0);
+        const __amdgpu_buffer_rsrc_t dr = ng_row(dx + (int64_t)(row < M ? row : 0) * d, dx && row < M ? bytes : 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float o[VEC];
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256) void norm_bwd_narrow_kernel(const T* __restric
         load(row0 + stride);
         c1 = sum16(c1) * inv_d;
         c2 = sum16(c2) * inv_d;
-        const __amdgpu_buffer_rsrc_t r = ro.at(dx, row0, M, d);
+        const __amdgpu_buffer_rsrc_t r = ro.at(dx, row0, dx ? M : 0, d);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float o[VEC];
@@ -628,7 +628,8 @@ int norm_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const float* ga
              float* dgamma, float* dbeta, float* ws, int M, int d, hipStream_t s) {
     const bool few = M <= NG_FEW;  // the row workgroups then have one turn of rows each
     const int turn = d <= NG_NARROW ? NG_NARROW_ROWS : ng_rows(ng_waves(d));
-    const int G = few ? (M + turn - 1) / turn : ng_groups(M, d), cols = few && (dgamma || dbeta) ? (d + 31) / 32 : 0;
+    const int cols = few && (dgamma || dbeta) ? (d + 31) / 32 : 0;
+    const int G = !few ? ng_groups(M, d) : dx ? (M + turn - 1) / turn : 0;  // few rows: the row workgroups are there for dx alone
     float* pg = dgamma ? (few ? dgamma : ws) : nullptr;
     float* pb = dbeta ? (few ? dbeta : ws + (int64_t)G * d) : nullptr;
     auto go = [&](auto vec, auto nv, auto wpr) {
@@ -685,7 +686,8 @@ extern "C" int esmk_layernorm_bwd(const void* dy, int64_t lddy, const void* x, i
         ESMK_CHECK_LAUNCH("esmk_layernorm_bwd");
         return ESMK_OK;
     }
-    if (!dy || !x || !gamma || !stats || !dx) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_bwd: null pointer");
+    if (!dy || !x || !gamma || !stats) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_bwd: null pointer");
+    if (!dx && !dgamma && !dbeta) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_bwd: null pointer (no gradient is wanted)");
     if (ldx < d || lddy < d) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_bwd: row stride below d=%d", d);
     if ((uintptr_t)stats & 7) ESMK_FAIL(ESMK_ERR_INVALID_ARG, "esmk_layernorm_bwd: stats must be 8-byte aligned");
     if ((dgamma || dbeta) && esmk_layernorm_bwd_workspace_bytes(M, d) > (workspace ? workspace_bytes : 0))

@@ -112,9 +112,10 @@ def layer_norm_forward(x, weight, bias=None, eps: float = 1e-5):
     return y, stats
 
 
-def layer_norm_backward(dy, x, weight, stats, bias: bool = True, param_grads: bool = True):
+def layer_norm_backward(dy, x, weight, stats, bias: bool = True, param_grads: bool = True, input_grad: bool = True):
     """Gradients of `layer_norm_forward` -> (dx, dweight, dbias).  dx has x's dtype, dweight and dbias are fp32 [d] sums over
-    all rows; dbias is None without `bias`, both are None without `param_grads` (a frozen norm)."""
+    all rows; dbias is None without `bias`, both are None without `param_grads` (a frozen norm), dx is None without `input_grad`
+    (a norm of fixed inputs)."""
     gpu, shape, M, d = _check_norm(x, weight, None)
     _need(dy, "dy", (x.dtype,), gpu)
     _need(stats, "stats", _F32, gpu)
@@ -123,13 +124,15 @@ def layer_norm_backward(dy, x, weight, stats, bias: bool = True, param_grads: bo
     xr, ldx = _rows(x, d)
     gr, ldg = _rows(dy, d)
     w = _param(weight)
-    dx = torch.empty_like(x, memory_format=_DENSE)
+    if not (input_grad or param_grads):
+        return None, None, None
+    dx = torch.empty_like(x, memory_format=_DENSE) if input_grad else None
     dw = w.new_empty(d) if param_grads else None
     db = w.new_empty(d) if param_grads and bias else None
     nbytes = L.lib().esmk_layernorm_bwd_workspace_bytes(M, d) if param_grads else 0
     ws = w.new_empty(nbytes // 4) if nbytes else None
     _call(gpu, "esmk_layernorm_bwd", gr.data_ptr(), ldg, xr.data_ptr(), ldx, _DTYPES[x.dtype], w.data_ptr(), stats.data_ptr(),
-          dx.data_ptr(), None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+          None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
           None if ws is None else ws.data_ptr(), nbytes, M, d)
     return dx, dw, db
 
@@ -146,10 +149,9 @@ class _LayerNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        want_w, want_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
-        dx, dw, db = layer_norm_backward(dy, x, weight, stats, bias=want_b, param_grads=want_w or want_b)
-        return (dx if ctx.needs_input_grad[0] else None, dw.to(weight.dtype) if want_w else None,
-                db.to(ctx.bias_dtype) if want_b else None, None)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx, dw, db = layer_norm_backward(dy, x, weight, stats, bias=want_b, param_grads=want_w or want_b, input_grad=want_x)
+        return dx, dw.to(weight.dtype) if want_w else None, db.to(ctx.bias_dtype) if want_b else None, None
 
 
 def layer_norm(x, weight, bias=None, eps: float = 1e-5):
@@ -227,9 +229,9 @@ def attention_varlen_forward(q, k, v, cu_seqlens, scale: float | None = None, ke
     return out, lse
 
 
-def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float | None = None, key_mask=None):
-    """Gradients of `attention_varlen_forward` -> (dq, dk, dv), dense bf16 in the shapes of q, k and v.  out and lse are the
-    forward call's, on the same inputs.  Probabilities and their gradients are rounded to bf16 for the products with q, k and
+def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float | None = None, key_mask=None, kv_grads: bool = True):
+    """Gradients of `attention_varlen_forward` -> (dq, dk, dv), dense bf16 in the shapes of q, k and v; dk and dv are None without
+    `kv_grads` (fixed keys and values).  out and lse are the forward call's, on the same inputs.  Probabilities and their gradients are rounded to bf16 for the products with q, k and
     dout; every sum is fp32, and shared key heads sum over their query heads in fp32.  Sequences of at most 64 unmasked keys
     lose nothing of dq and dk but the rounding of the results: delta is summed without the rounding of out, and the gradients of
     the probabilities enter in two bf16 parts.  That depends on a sequence's own keys, not on padding or on the rest of the
@@ -246,10 +248,12 @@ def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float 
     dout, gp, gt, gh = _strided(dout, "dout")
     (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = _strided(q, "q"), _strided(k, "k"), _strided(v, "v")
     out, op, ot, oh = _strided(out, "out")
-    dq, dk, dv = (torch.empty_like(t, memory_format=_DENSE) for t in (q, k, v))
+    dq = torch.empty_like(q, memory_format=_DENSE)
+    dk, dv = (torch.empty_like(t, memory_format=_DENSE) if kv_grads else None for t in (k, v))
     nbytes = L.lib().esmk_attn_varlen_bwd_workspace_bytes(N, H)
     ws = lse.new_empty(nbytes // 4)
-    _call(gpu, "esmk_attn_varlen_bwd", gp, qp, kp, vp, op, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    _call(gpu, "esmk_attn_varlen_bwd", gp, qp, kp, vp, op, lse.data_ptr(), dq.data_ptr(),
+          None if dk is None else dk.data_ptr(), None if dv is None else dv.data_ptr(),
           _Strides16(gt, gh, qt, qh, kt, kh, vt, vh, ot, oh, H * D, D, G * D, D, G * D, D), cu_seqlens.data_ptr(),
           cu_seqlens.numel() - 1, None if key_mask is None else key_mask.data_ptr(), N, H, G, D, scale, ws.data_ptr(), nbytes)
     return dq, dk, dv
@@ -267,7 +271,8 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, cu_seqlens, key_mask = ctx.saved_tensors
-        return (*attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, ctx.scale, key_mask), None, None, None)
+        return (*attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, ctx.scale, key_mask,
+                                           kv_grads=any(ctx.needs_input_grad[1:3])), None, None, None)
 
 
 def attention_varlen(q, k, v, cu_seqlens, scale: float | None = None, key_mask=None):

@@ -256,7 +256,7 @@ int esmk_attn_l64_d128(const void* qkv_bf16, void* ctx_bf16, const float* rope_c
  * address that suits the type.  stats 8-byte aligned. */
 int esmk_layernorm_fwd(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, void* y, float* stats,
                        int M, int d, float eps, esmk_stream_t stream);
-/* dx [M, d] (dtype, dense rows); dgamma, dbeta f32 [d], overwritten (either may be NULL: not wanted).  dy, x: dtype, rows
+/* dx [M, d] (dtype, dense rows); dgamma, dbeta f32 [d], overwritten.  Any of the three may be NULL: not wanted.  dy, x: dtype, rows
  * lddy / ldx >= d elements apart; stats from esmk_layernorm_fwd.  workspace: esmk_layernorm_bwd_workspace_bytes (needed
  * only where dgamma or dbeta is).  M = 0 sets dgamma and dbeta to zero. */
 size_t esmk_layernorm_bwd_workspace_bytes(int M, int d);
@@ -276,7 +276,8 @@ int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v, void* out,
                          const int32_t* cu_seqlens, int n_segments, const uint8_t* key_mask, int n_tokens, int n_heads,
                          int n_kv_heads, int head_dim, float scale, esmk_stream_t stream);
 /* Gradients of the same with respect to q, k and v, from out and lse of esmk_attn_varlen_fwd on the same inputs.  strides:
- * 16 values for dout, q, k, v, out, dq, dk, dv.  dk and dv are summed over the query heads that share a key head.  Masked
+ * 16 values for dout, q, k, v, out, dq, dk, dv.  dk and dv are summed over the query heads that share a key head; both may be
+ * NULL: not wanted.  Masked
  * keys, queries without a key and tokens in no sequence get zeros.  Probabilities and their gradients are rounded to bf16 for
  * the second products; in sequences of at most 64 unmasked keys the gradients enter in two parts, and rowsum(dout out) is summed
  * again without the rounding of out.  workspace: esmk_attn_varlen_bwd_workspace_bytes, owned by this call while it runs. */

@@ -133,6 +133,70 @@ def test_layer_norm_slices_of_wider_activations(d, dtype):
         assert torch.equal(leaf.grad.reshape(-1, d), want[2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d", [(1, 64), (200, 65), (512, 256), (513, 256), (3000, 129), (300, 960), (512, 12288), (600, 1152), (2049, 1281),
+                                    (700, 6145)])
+def test_layer_norm_each_gradient_alone(rows, d, dtype):
+    """What is not wanted changes no bit of what is: input and parameter gradients alone, one parameter's alone (C interface)."""
+    from esm_amd import _lib as L
+    g = gen(rows + d)
+    x, dy = randn(g, rows, d).to(dtype), randn(g, rows, d).to(dtype)
+    w, b = 1 + 0.1 * randn(g, d), randn(g, d)
+    y, st = T().layer_norm_forward(x, w, b)
+    dx, dw, db = T().layer_norm_backward(dy, x, w, st)
+    want, tol = norm_oracle(x, w, b, dy)
+    for got, a, t in zip((dx, dw, db), want[1:], tol[1:]):
+        within(got, a, t, "all")
+    none = T().layer_norm_backward(dy, x, w, st, param_grads=False)
+    assert torch.equal(none[0], dx) and none[1] is None and none[2] is None
+    par = T().layer_norm_backward(dy, x, w, st, input_grad=False)
+    assert par[0] is None and torch.equal(par[1], dw) and torch.equal(par[2], db)
+    assert T().layer_norm_backward(dy, x, w, st, param_grads=False, input_grad=False) == (None, None, None)
+    nbytes = L.lib().esmk_layernorm_bwd_workspace_bytes(rows, d)
+    for with_x in (True, False):
+        for p, q in ((dw, None), (None, db)):
+            ws = torch.empty(nbytes // 4 + 1, device="cuda")
+            gx, gw, gb = (None if t is None else torch.full_like(t, 7.0) for t in (dx if with_x else None, p, q))
+            L.check(L.lib().esmk_layernorm_bwd(dy.data_ptr(), d, x.data_ptr(), d, 0 if dtype is torch.float32 else 1, w.data_ptr(), st.data_ptr(),
+                                               L.ptr(gx), L.ptr(gw), L.ptr(gb), ws.data_ptr(), nbytes, rows, d,
+                                               torch.cuda.current_stream().cuda_stream))
+            for got, full in ((gx, dx), (gw, dw), (gb, db)):
+                assert got is None or torch.equal(got, full)
+
+
+def test_autograd_asks_for_no_gradient_that_is_not_wanted(monkeypatch):
+    """Frozen inputs and parameters: the call is told, and what is asked for keeps its bits."""
+    t = T()
+    calls = []
+    call = t._call
+    monkeypatch.setattr(t, "_call", lambda gpu, name, *args: (calls.append((name, args)), call(gpu, name, *args))[1])
+    g = gen(12)
+    x, w, b, dy = randn(g, 700, 96), 1 + 0.1 * randn(g, 96), randn(g, 96), randn(g, 700, 96)
+    y, st = t.layer_norm_forward(x, w, b)
+    full = t.layer_norm_backward(dy, x, w, st)
+    for wants in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 1, 1)):
+        leaves = [u.clone().requires_grad_(bool(v)) for u, v in zip((x, w, b), wants)]
+        t.layer_norm(*leaves).backward(dy)
+        name, args = calls[-1]
+        assert name == "esmk_layernorm_bwd" and [a is not None for a in args[7:10]] == [wants[0] == 1, wants[1] + wants[2] > 0, wants[2] == 1]
+        for leaf, want in zip(leaves, full):
+            assert leaf.grad is None if not leaf.requires_grad else torch.equal(leaf.grad, want)
+    row = x[:1].clone().requires_grad_()  # a broadcast input's gradient is summed
+    t.layer_norm(row.expand(700, 96), w, b).backward(dy)
+    dx = t.layer_norm_backward(dy, x[:1].expand(700, 96), w, t.layer_norm_forward(x[:1].expand(700, 96), w)[1])[0]
+    assert torch.equal(row.grad, dx.sum(0, keepdim=True))
+    for r in (1, 70):  # few blocks and many
+        q, k, v, cu, cut, dout, _ = attention_inputs(19, [130, 31, 64], 2 * r, r, 64, tail=2)
+        full = attention_all(q, k, v, cut, dout)[2:]
+        for wants in ((1, 0, 0), (1, 1, 0), (0, 0, 1), (1, 1, 1)):
+            leaves = [u.clone().requires_grad_(bool(a)) for u, a in zip((q, k, v), wants)]
+            t.attention_varlen(*leaves, cut).backward(dout)
+            name, args = calls[-1]
+            assert name == "esmk_attn_varlen_bwd" and [a is not None for a in args[6:9]] == [True] + 2 * [wants[1] + wants[2] > 0]
+            for leaf, want in zip(leaves, full):
+                assert leaf.grad is None if not leaf.requires_grad else torch.equal(leaf.grad, want)
+
+
 def test_layer_norm_no_rows_gives_zero_parameter_gradients():
     x, w = torch.empty(0, 96, device="cuda"), torch.ones(96, device="cuda")
     y, st = T().layer_norm_forward(x, w)

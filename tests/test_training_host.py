@@ -38,6 +38,7 @@ def test_layernorm_entry_points_refuse():
     refused(bwd(M=2 ** 30 + 1), UNSUPPORTED, "M=1073741825")
     refused(bwd(ws=None), WORKSPACE, "workspace")
     refused(bwd(nb=lib.esmk_layernorm_bwd_workspace_bytes(4096, 64) - 1), WORKSPACE, "workspace")
+    refused(lib.esmk_layernorm_bwd(P, 64, P, 64, L.BF16, P, P, None, None, None, P, 1 << 30, 4096, 64, None), INVALID, "no gradient")
     assert lib.esmk_layernorm_bwd_workspace_bytes(512, 12288) == 0 and lib.esmk_layernorm_bwd_workspace_bytes(513, 64) > 0
     assert lib.esmk_layernorm_bwd_workspace_bytes(0, 64) == 0 and lib.esmk_layernorm_bwd_workspace_bytes(4096, 64) > 0
 
@@ -72,6 +73,9 @@ def test_attention_entry_points_refuse():
     refused(bwd(st=(128, 64) * 7 + (4, 64)), INVALID, "tensor 7")
     refused(bwd(ws=None), WORKSPACE, "32 workspace")
     refused(bwd(nb=31), WORKSPACE, "32 workspace")
+    for dk, dv in ((None, P), (P, None)):
+        refused(lib.esmk_attn_varlen_bwd(P, P, P, P, P, P, P, dk, dv, (C.c_int64 * 16)(*(128, 64) * 8), P, 1, None, 4, 2, 2, 64, 0.125, P, 1 << 20,
+                                         None), INVALID, "together")
 
 
 def test_preference_entry_points_refuse():
