@@ -28,6 +28,15 @@ _Strides8, _Strides16 = C.c_int64 * 8, C.c_int64 * 16
 Tensor, _DENSE = torch.Tensor, torch.contiguous_format
 
 
+def _public_stream(gpu):
+    return torch.cuda.current_stream(gpu).cuda_stream
+
+
+# The current stream's handle.  torch's compiler-facing call spares the Stream object around it, 1 us of a small operator's 8 on the
+# host; a torch without that call is asked the public way.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
+
+
 def _need(t, name, dtypes, gpu=None):
     """`t` has to be a tensor of one of `dtypes` on a GPU (on that one, if given)."""
     if isinstance(t, Tensor) and t.dtype in dtypes and t.is_cuda and (gpu is None or t.get_device() == gpu):
@@ -42,13 +51,12 @@ def _need(t, name, dtypes, gpu=None):
 
 
 def _call(gpu, name, *args):
-    """One C entry point on the tensors' GPU and its current stream.  The calls are short: half of a small operator's time
-    is spent on this side of them, so the raw stream handle is taken without building a Stream object."""
-    if gpu == torch._C._cuda_getDevice():
-        rc = getattr(L.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(gpu))
+    """One C entry point on the tensors' GPU and its current stream."""
+    if gpu == torch.cuda.current_device():
+        rc = getattr(L.lib(), name)(*args, _stream(gpu))
     else:
         with torch.cuda.device(gpu):
-            rc = getattr(L.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(gpu))
+            rc = getattr(L.lib(), name)(*args, _stream(gpu))
     if rc:
         L.check(rc, name)
 

@@ -935,6 +935,14 @@ def test_same_bits_again_on_other_streams_and_in_a_replayed_graph():
                 assert torch.equal(p, q)
 
 
+def test_the_stream_of_a_call_is_the_current_one():
+    gpu = torch.cuda.current_device()
+    side = torch.cuda.Stream()
+    for s in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(s):
+            assert T()._stream(gpu) == T()._public_stream(gpu) == s.cuda_stream
+
+
 @pytest.mark.parametrize("H,G", [(2, 1), (150, 75)])
 def test_attention_graph_follows_the_offsets(H, G):
     """The order of the blocks is formed on the GPU: a captured step holds for other offsets, with few blocks and with many."""

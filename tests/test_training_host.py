@@ -1,5 +1,7 @@
 """Training operators without a GPU: what the C entry points and their Python callers refuse before any launch."""
 import ctypes as C
+import importlib.util
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -136,3 +138,16 @@ def test_rows_of_wider_tensors_are_read_in_place():
               qkv[:1, :, :16].expand(3, 7, 16), qkv[0, :1, :16].expand(7, 16), torch.zeros(40).as_strided((5, 8), (4, 1))):
         rows, got = T._rows(t, t.shape[-1])
         assert rows.is_contiguous() and rows.data_ptr() != t.data_ptr() and got == t.shape[-1] and torch.equal(rows, t)
+
+
+def test_a_torch_without_the_raw_stream_call_is_asked_for_its_stream(monkeypatch):
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    spec = importlib.util.spec_from_file_location("esm_amd.training_again", T.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda gpu: SimpleNamespace(cuda_stream=100 + gpu))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    sent = []
+    monkeypatch.setattr(L, "lib", lambda: SimpleNamespace(esmk_some_call=lambda *a: sent.append(a) or 0))
+    again._call(3, "esmk_some_call", 1, 2)
+    assert sent == [(1, 2, 103)]
