@@ -446,13 +446,13 @@ struct OwnRow {
 //   * puts dS into its products in two bf16 parts.
 // dq of 2, 4 and 16 keys (among 130 tokens) is off by 4.0e-3, 3.0e-3, 2.2e-3 of its norm without the first; of 64 keys by 2.4e-3
 // without the second; with both by 1.7e-3, which is the rounding of dq alone.  Backward pass of 500 sequences of 64 tokens, 18
-// heads: 216 and 234 us.  For sequences of up to 512 keys the second part would make 64 x 512 tokens 354 -> 486 us.
+// heads: 215 and 226 us.  For sequences of up to 512 keys the second part would make 64 x 512 tokens 354 -> 486 us.
 // The rule looks at the sequence's own keys alone: a padded row's gradients are as exact as the packed sequence's, whatever else
 // is in the call.
 constexpr int AG_FEW_KEYS = 64;
 
 // Masked sequences count 512 keys at a time and stop behind the 64th, so that all but very sparse masks cost one read (64 x 512
-// tokens with a mask, backward pass: 364 and 371 us).
+// tokens with a mask, backward pass: 359 and 365 us).
 __device__ __forceinline__ bool few_keys(const unsigned char* mask, const Span& sp, int lane) {
     if (!mask || sp.len <= AG_FEW_KEYS) return sp.len <= AG_FEW_KEYS;
     int n = 0;
@@ -724,9 +724,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dq_ke
 // At head dim 128 the accumulators take 128 registers and K's fragments 32; V's would leave one wave per SIMD, so they are
 // read from LDS where they are used (LDS reads run at 256 bytes a cycle, a third of the time unused), and the ring holds
 // 32-row tiles: 64 KiB a workgroup, two of them on a CU.
-// Both head dims run at their register limit.  The loops over full tiles use no scratch (the lane's row is worked out again at the
-// store, and the path of few keys is a body of its own); a few registers are kept in it around them, and about nine in the loop of
-// few keys (500 x 64 tokens, 18 heads, backward pass 234 us; with twice as many of them 365).
+// Both head dims run at their register limit.  The loops over full tiles use no scratch: the lane's row is worked out again at the
+// store, and the path of few keys is a body of its own that forms one product at a time (with 24 spilled registers in its loop, 500 x
+// 64 tokens, 18 heads took 365 us, backward pass, instead of 226).  Head dim 64 keeps 24 bytes a lane in it around the loops.
 constexpr int dkdv_rt(int D) { return D == 128 ? 32 : 64; }  // rows of a streamed tile
 
 template <int D, bool FEW>
@@ -780,6 +780,9 @@ __device__ __forceinline__ void dkdv_rows(const View& dout, const View& q, const
     const float inv_scale = 1.0f / scale;
     float next = 0.f;
     int gq = 0, qt = 0;  // head of the group and tile that stage() takes next
+    // of rows past the end; a scalar: kept per lane it was read from scratch in the loop at D 128, and waiting for that waits for the
+    // tile in flight too (8 x 2048 tokens, 16 heads, backward pass 980 -> 1050 us)
+    const int none = __builtin_amdgcn_readfirstlane(wave ? 0 : 0x7f800000);
     auto stage = [&](int slot) {
         const int left = sp.len - qt * RT, head = kvh * group + gq;
         const int64_t t0 = sp.s0 + (int64_t)qt * RT;
@@ -788,7 +791,7 @@ __device__ __forceinline__ void dkdv_rows(const View& dout, const View& q, const
         sg.go(base + TILE, dout.p + t0 * dout.tok + head * dout.head, left, wave);
         if (wave < 2) {  // wave 0: lse, wave 1: delta.  Rows past the end get probability 2^-inf = 0
             const float* src = (wave ? delta : lse) + (int64_t)head * N + t0;
-            const float x = lane < left && lane < RT ? src[lane] : (wave ? 0.f : INFINITY);
+            const float x = lane < left && lane < RT ? src[lane] : __int_as_float(none);
             next = wave ? -x : -x * inv_scale;
         }
         if (++qt == nt) { qt = 0; ++gq; }
@@ -801,10 +804,9 @@ __device__ __forceinline__ void dkdv_rows(const View& dout, const View& q, const
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
     const float c = scale * AG_LOG2E;
 
-    auto half = [&](auto mt_, int cur, const float* st) {
+    auto dp_of = [&](auto mt_, int cur, const float* st) {  // dO V^T - delta
         constexpr int mt = decltype(mt_)::value;
-        const f32x16 s = mfma_rows<D>(smem + cur + mt * 64 * D, koff, kf, rows16(st, mt, hi));  // Q K^T - lse / scale
-        f32x16 dp = rows16(st + RT, mt, hi);                                          // dO V^T - delta
+        f32x16 dp = rows16(st + RT, mt, hi);
         if constexpr (VL) {
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
@@ -813,19 +815,32 @@ __device__ __forceinline__ void dkdv_rows(const View& dout, const View& q, const
         } else {
             dp = mfma_rows<D>(smem + cur + TILE + mt * 64 * D, koff, vf, dp);
         }
+        return dp;
+    };
+    auto half = [&](auto mt_, int cur, const float* st) {
+        constexpr int mt = decltype(mt_)::value;
+        const f32x16 s = mfma_rows<D>(smem + cur + mt * 64 * D, koff, kf, rows16(st, mt, hi));  // Q K^T - lse / scale
         float e[16], f[16];
+        if constexpr (FEW) {  // one product at a time: registers
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(s[r] * c);
-            f[r] = e[r] * dp[r];
-        }
-        // 2^-8 relative at most, for the products with dO and Q
-        const bf16x8 p[2] = {pack8(e), pack8(e + 8)};
-        if constexpr (FEW) {
+            for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(s[r] * c);
+            const bf16x8 p[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with dO
+            __builtin_amdgcn_sched_barrier(0);
             mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
+            __builtin_amdgcn_sched_barrier(0);
+            const f32x16 dp = dp_of(mt_, cur, st);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) f[r] = e[r] * dp[r];
             mfma_tr_two<D, mt>(ak, ta, lds0 + cur, f);
         } else {
-            const bf16x8 ds[2] = {pack8(f), pack8(f + 8)};
+            const f32x16 dp = dp_of(mt_, cur, st);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                e[r] = __builtin_amdgcn_exp2f(s[r] * c);
+                f[r] = e[r] * dp[r];
+            }
+            // 2^-8 relative at most, for the products with dO and Q
+            const bf16x8 p[2] = {pack8(e), pack8(e + 8)}, ds[2] = {pack8(f), pack8(f + 8)};
             mfma_tr<D, mt>(av, ta, lds0 + cur + TILE, p);
             mfma_tr<D, mt>(ak, ta, lds0 + cur, ds);
         }
@@ -867,8 +882,8 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
     if (!find_span(od, cu, n_seg, N, kvh, sp)) return;
     const OwnRow r(sp, wave, lane);
     const bool live = r.on && !sp.dead && (!mask || mask[r.tok]);
-    const bool few = few_keys(mask, sp, lane);
-    if (!__syncthreads_or(live)) {  // no key of the block takes part
+    const int keys = __syncthreads_count(live) / 2;  // two lanes a row
+    if (keys == 0) {  // no key of the block takes part
         f32x16 z[D / 32];
 #pragma unroll
         for (int t = 0; t < D / 32; ++t) z[t] = splat16(0.f);
@@ -876,7 +891,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
         store_row<D>(dv.p + r.tok * dv.tok + kvh * dv.head, z, 0.f, lane >> 5, r.on);
         return;
     }
-    if (few) dkdv_rows<D, true>(dout, q, k, v, lse, delta, dk, dv, N, group, scale, kvh, sp, live, smem, stat, wave, lane);
+    if (keys <= AG_FEW_KEYS && few_keys(mask, sp, lane)) dkdv_rows<D, true>(dout, q, k, v, lse, delta, dk, dv, N, group, scale, kvh, sp, live, smem, stat, wave, lane);
     else dkdv_rows<D, false>(dout, q, k, v, lse, delta, dk, dv, N, group, scale, kvh, sp, live, smem, stat, wave, lane);
 }
 
