@@ -15,7 +15,8 @@
 // second product is read from the same row-major tile with ds_read_b64_tr_b16: the LDS image's 16-byte chunks are
 // XOR-swizzled by a function of the row that keeps both the row reads and the transposed reads free of bank conflicts.
 //
-// Calls with no more blocks of 128 rows than CUs run smaller blocks, whose four waves share the other side ("few rows" below).
+// Calls whose blocks of 128 rows do not fill the card run smaller blocks, whose four waves share the other side ("few rows" below,
+// ag_few()).
 //
 // The backward pass is two kernels, each with one owner for every output element (no atomics, so the same inputs give the
 // same bits): dQ per query block (three products; it also forms delta), dK / dV per key block (four).
@@ -899,10 +900,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
 // Where the blocks of 128 rows do not fill the card, a workgroup owns 32 rows and its four waves take every fourth tile of the
 // other side, each through a ring of its own and without a barrier; at the end their sums are joined in LDS, in the order of
 // the waves.  Four times the workgroups, each a quarter as long; four times the tile loads.  One path for all masks.
-// Forward and backward pass, blocks of 128 rows and this (blocks of 128, us): one sequence of 4096, a head of 64: 35 blocks, 67, 184
-// and 39, 78; 4 heads: 140, 72, 190 and 49, 102; 3 of 2652, 3 heads: 201, 62, 150 and 63, 128; one of 4096, 8 heads: 280, 76, 199 and
-// 85, 183; 12 heads: 420, 92, 248 and 118, 262; heads of 128, 2: 70, 104, 323 and 56, 134; 8: 280, 118, 356 and 181, 449.  3 of 2652,
-// 4 : 1 heads of 128, where only dK dV is short of blocks (67): backward pass 582 and 248.
+// Forward and backward pass, blocks of 128 rows and this (us): one sequence of 4096, a head of 64: 67, 184 and 39, 78; 4 heads: 72,
+// 190 and 49, 102; 3 of 2652, 4 : 1 heads of 128, where only dK dV is short of blocks: backward pass 582 and 248.  ag_few() has the
+// bounds and what was measured around them.
 
 // Sum of the four waves' accumulators [column 32 t + crow(r, hi)][row on the lane], each times its `mul`, written as bf16 rows.
 // All waves have to be done with `area`.
@@ -1252,8 +1252,18 @@ Order ag_order(int N, int n_seg, int heads, int blk = AG_BLK) {
     if (o.even) o.grid = o.n_blk * heads;
     return o;
 }
-// No more blocks of 128 rows than CUs.
-bool ag_few(int N, int n_seg, int heads) { return (N / AG_BLK + n_seg + 2) * (long long)heads <= 256; }
+// Blocks of 32 rows where there are few of 128, block numbers without rows counted: no more than CUs at head dim 64, where a CU holds
+// two workgroups of 32 rows, and 144 at 128, where their rings leave one on a CU.  A workgroup of 32 rows takes a quarter of the time
+// only where each wave has several tiles, so that sequences below 512 tokens on average have to fit at once as well.
+// Forward and backward pass, blocks of 128 rows and of 32 (us).  Head dim 64, blocks: one of 4096, 210: 69, 187 and 66, 153; 245: 72, 189
+// and 73, 169; 280: 59, 168 and 70, 165.  12 of 300, 168 (496 workgroups of 32 rows): 10.5, 22.7 and 10.4, 19.0; 210 (620): 10.5, 24.6
+// and 14.0, 33.5.  Head dim 128: one of 4096, 140: 96, 318 and 88, 239; 175: 123, 324 and 139, 359; 245: 123, 324 and 184, 477.  8 of 512,
+// 84: 15.8, 51.0 and 10.9, 31.0; 126: 19.1, 52.7 and 21.0, 58.4, the most it loses.  12 of 300, 168: 11.7, 36.8 and 15.9, 45.5.
+bool ag_few(int N, int n_seg, int heads, int D) {
+    const int per_cu = D == 64 ? 2 : 1;
+    if ((N / AG_BLK + n_seg + 2) * (long long)heads > (D == 64 ? 256 : 144)) return false;
+    return N / EVEN_LONG >= n_seg || (N / AG_FEW_BLK + n_seg) * (long long)heads <= 256 * per_cu;
+}
 
 bool ag_strides(const void* p, const int64_t* st, int D) {
     // 16-byte rows; a tile's offsets (64 rows) stay inside the 31 bits of a buffer descriptor
@@ -1286,7 +1296,7 @@ extern "C" int esmk_attn_varlen_fwd(const void* q, const void* k, const void* v,
     const View vq{(const __bf16*)q, strides[0], strides[1]}, vk{(const __bf16*)k, strides[2], strides[3]}, vv{(const __bf16*)v, strides[4], strides[5]};
     const OutView vo{(__bf16*)out, strides[6], strides[7]};
     const int group = n_heads / n_kv_heads;
-    const bool few = ag_few(n_tokens, n_segments, n_heads);
+    const bool few = ag_few(n_tokens, n_segments, n_heads, head_dim);
     const Order od = ag_order(n_tokens, n_segments, n_heads, few ? AG_FEW_BLK : AG_BLK);
     auto* kern = few             ? (head_dim == 64 ? attn_fwd_few_kernel<64> : attn_fwd_few_kernel<128>)
                  : head_dim == 64 ? (key_mask ? attn_fwd_lse_kernel<64, true> : attn_fwd_lse_kernel<64, false>)
@@ -1319,7 +1329,7 @@ extern "C" int esmk_attn_varlen_bwd(const void* dout, const void* q, const void*
     auto in = [&](int i) { return View{(const __bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
     auto ov = [&](int i) { return OutView{(__bf16*)ps[i], strides[2 * i], strides[2 * i + 1]}; };
     const int group = n_heads / n_kv_heads;
-    const bool few_q = ag_few(n_tokens, n_segments, n_heads), few_k = ag_few(n_tokens, n_segments, n_kv_heads);
+    const bool few_q = ag_few(n_tokens, n_segments, n_heads, head_dim), few_k = ag_few(n_tokens, n_segments, n_kv_heads, head_dim);
     const Order oq = ag_order(n_tokens, n_segments, n_heads, few_q ? AG_FEW_BLK : AG_BLK);
     const Order ok = ag_order(n_tokens, n_segments, n_kv_heads, few_k ? AG_FEW_BLK : AG_BLK);
     float* delta = (float*)workspace;
