@@ -21,9 +21,9 @@
 // The backward pass is two kernels, each with one owner for every output element (no atomics, so the same inputs give the
 // same bits): dQ per query block (three products; it also forms delta), dK / dV per key block (four).
 //
-// Measured (forward, dQ, dK dV): 64 x 512 tokens, 18 heads of 64: 115, 174, 220 us - eight tiles per workgroup, so that a third
-// of its life is the load of the first rows and the store of the last; 4 x 4096, 40 heads of 64: 715, 970, 1271 us (961, 1063,
-// 1081 TFLOP/s) - matrix pipes 54 to 60 % busy at the clock the power limit leaves; a 2 TB/s share of HBM in both.
+// Measured (forward, dQ, dK dV): 64 x 512 tokens, 18 heads of 64: 113, 170, 221 us - eight tiles per workgroup, so that a third
+// of its life is the load of the first rows and the store of the last; 4 x 4096, 40 heads of 64: 691, 936, 1246 us (995, 1101,
+// 1103 TFLOP/s) - matrix pipes 55 to 60 % busy at the clock the power limit leaves; a 2 TB/s share of HBM in both.
 #include <math.h>
 
 #include <type_traits>

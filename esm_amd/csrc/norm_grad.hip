@@ -5,7 +5,7 @@
 //   g = dy gamma,  dx = rstd (g - mean_d(g) - h mean_d(g h)),  dgamma = sum_rows dy h,  dbeta = sum_rows dy
 //
 // Both are bound by HBM: the forward pass has to move 2 M d elements, the backward pass 3 M d.  At 32768 x 1152 bf16 the
-// forward pass takes 30 us (5.0 TB/s; a copy of the same size 5.0), the backward pass 42 + 5 us (5.4 TB/s).  WPR waves share a row
+// forward pass takes 30 us (5.0 TB/s; a copy of the same size 5.0), the backward pass 39 + 5 us (5.8 TB/s).  WPR waves share a row
 // and keep all of it in registers (one read), sums run in fp32, and the next row's loads are in flight while the current
 // one is reduced.  A lane owns the same columns of every row it meets, so it sums its columns of dgamma / dbeta in
 // registers; each workgroup leaves one partial row, and a second kernel adds the partial rows in a fixed order (no

@@ -1,4 +1,4 @@
-"""Operators for fine-tuning the trunk: LayerNorm, block-diagonal attention and a paired preference loss, each with its
+"""Operators for fine-tuning: LayerNorm, block-diagonal attention and a paired preference loss, each with its
 gradient, on hand-written gfx950 kernels (include/esmk.h, "Training").
 
 Every operator comes in two forms:
@@ -9,8 +9,9 @@ Every operator comes in two forms:
 Tensors live on one GPU; work is enqueued on that GPU's current stream and nothing waits for it.  Outputs and scratch memory
 come from torch's allocator.  Wrong shapes, types or devices raise ValueError / TypeError before anything is launched.
 
-The reference differentiates its own modules (esm/layers/attention.py:26-33,65-78, esm/layers/blocks.py:31) through
-autograd; the loss has no counterpart there.
+The models' own forward passes keep no graph: a program that trains writes its blocks from these operators and torch's.  The
+reference differentiates its own modules (esm/layers/attention.py:26-33,65-78, esm/layers/blocks.py:31) through autograd; the
+loss has no counterpart there.
 """
 from __future__ import annotations
 
@@ -310,7 +311,7 @@ def preference_loss_forward(logits, targets, cu_seqlens, ref_logps, beta: float 
                             nll_weight: float = 0.0):
     """Preference loss of packed sequence pairs -> (loss, logps, saved).
 
-    logits [N, V] fp32 or bf16 over the packed tokens; targets int64 [N], a value outside [0, V) marks a token that is not
+    logits [N, V] fp32 or bf16 over the packed tokens (copied where they are not dense); targets int64 [N], a value outside [0, V) marks a token that is not
     scored; cu_seqlens int32 [2 P + 1]: sequences 2i (preferred) and 2i + 1 (other) are pair i; ref_logps fp32 [2 P] the
     frozen model's log-probabilities.
         logps[s] = sum over scored tokens of log softmax(logits)[target]
