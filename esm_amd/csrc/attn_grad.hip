@@ -900,9 +900,9 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 3 : 2) void attn_bwd_dkdv_
 // Where the blocks of 128 rows do not fill the card, a workgroup owns 32 rows and its four waves take every fourth tile of the
 // other side, each through a ring of its own and without a barrier; at the end their sums are joined in LDS, in the order of
 // the waves.  Four times the workgroups, each a quarter as long; four times the tile loads.  One path for all masks.
-// Forward and backward pass, blocks of 128 rows and this (us): one sequence of 4096, a head of 64: 67, 184 and 39, 78; 4 heads: 72,
-// 190 and 49, 102; 3 of 2652, 4 : 1 heads of 128, where only dK dV is short of blocks: backward pass 582 and 248.  ag_few() has the
-// bounds and what was measured around them.
+// Forward and backward pass, blocks of 128 rows and this (us): one sequence of 4096, 4 heads of 64: 59, 169 and 40, 92; 3 of 2652, 4 : 1
+// heads of 128, where only dK dV is short of blocks: backward pass 582 and 248.  ag_few() has the bounds and what was measured
+// around them.
 
 // Sum of the four waves' accumulators [column 32 t + crow(r, hi)][row on the lane], each times its `mul`, written as bf16 rows.
 // All waves have to be done with `area`.
@@ -1258,7 +1258,8 @@ Order ag_order(int N, int n_seg, int heads, int blk = AG_BLK) {
 // Forward and backward pass, blocks of 128 rows and of 32 (us).  Head dim 64, blocks: one of 4096, 210: 69, 187 and 66, 153; 245: 72, 189
 // and 73, 169; 280: 59, 168 and 70, 165.  12 of 300, 168 (496 workgroups of 32 rows): 10.5, 22.7 and 10.4, 19.0; 210 (620): 10.5, 24.6
 // and 14.0, 33.5.  Head dim 128: one of 4096, 140: 96, 318 and 88, 239; 175: 123, 324 and 139, 359; 245: 123, 324 and 184, 477.  8 of 512,
-// 84: 15.8, 51.0 and 10.9, 31.0; 126: 19.1, 52.7 and 21.0, 58.4, the most it loses.  12 of 300, 168: 11.7, 36.8 and 15.9, 45.5.
+// 84: 15.8, 51.0 and 10.9, 31.0; 126: 19.1, 52.7 and 21.0, 58.4.  One of 700, 144: 20.4, 63.7 and 23.4, 64.9; these two are what it
+// loses most on.  12 of 300, 168: 11.7, 36.8 and 15.9, 45.5.
 bool ag_few(int N, int n_seg, int heads, int D) {
     const int per_cu = D == 64 ? 2 : 1;
     if ((N / AG_BLK + n_seg + 2) * (long long)heads > (D == 64 ? 256 : 144)) return false;

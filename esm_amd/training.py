@@ -1,5 +1,5 @@
-"""Operators for fine-tuning: LayerNorm, block-diagonal attention and a paired preference loss, each with its
-gradient, on hand-written gfx950 kernels (include/esmk.h, "Training").
+"""Operators for fine-tuning: LayerNorm, block-diagonal attention and a paired preference loss, each with its gradient, on
+hand-written gfx950 kernels (include/esmk.h, "Training").
 
 Every operator comes in two forms:
   * `layer_norm`, `attention_varlen`, `preference_loss`: differentiable, for torch's autograd;
@@ -238,13 +238,14 @@ def attention_varlen_forward(q, k, v, cu_seqlens, scale: float | None = None, ke
     return out, lse
 
 
-def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float | None = None, key_mask=None, kv_grads: bool = True):
+def attention_varlen_backward(dout, q, k, v, out, lse, cu_seqlens, scale: float | None = None, key_mask=None,
+                              kv_grads: bool = True):
     """Gradients of `attention_varlen_forward` -> (dq, dk, dv), dense bf16 in the shapes of q, k and v; dk and dv are None without
-    `kv_grads` (fixed keys and values).  out and lse are the forward call's, on the same inputs.  Probabilities and their gradients are rounded to bf16 for the products with q, k and
-    dout; every sum is fp32, and shared key heads sum over their query heads in fp32.  Sequences of at most 64 unmasked keys
-    lose nothing of dq and dk but the rounding of the results: delta is summed without the rounding of out, and the gradients of
-    the probabilities enter in two bf16 parts.  That depends on a sequence's own keys, not on padding or on the rest of the
-    call."""
+    `kv_grads` (fixed keys and values).  out and lse are the forward call's, on the same inputs.  Probabilities and their
+    gradients are rounded to bf16 for the products with q, k and dout; every sum is fp32, and shared key heads sum over their
+    query heads in fp32.  Sequences of at most 64 unmasked keys lose nothing of dq and dk but the rounding of the results:
+    rowsum(dout out) is summed without the rounding of out, and the gradients of the probabilities enter in two bf16 parts.  That
+    depends on a sequence's own keys, not on padding or on the rest of the call."""
     gpu, N, H, G, D = _check_attention(q, k, v, cu_seqlens, key_mask)
     scale = _scale(scale, D)
     _need(dout, "dout", _BF16, gpu)
@@ -311,9 +312,9 @@ def preference_loss_forward(logits, targets, cu_seqlens, ref_logps, beta: float 
                             nll_weight: float = 0.0):
     """Preference loss of packed sequence pairs -> (loss, logps, saved).
 
-    logits [N, V] fp32 or bf16 over the packed tokens (copied where they are not dense); targets int64 [N], a value outside [0, V) marks a token that is not
-    scored; cu_seqlens int32 [2 P + 1]: sequences 2i (preferred) and 2i + 1 (other) are pair i; ref_logps fp32 [2 P] the
-    frozen model's log-probabilities.
+    logits [N, V] fp32 or bf16 over the packed tokens (copied where they are not dense); targets int64 [N], a value outside
+    [0, V) marks a token that is not scored; cu_seqlens int32 [2 P + 1]: sequences 2i (preferred) and 2i + 1 (other) are pair
+    i; ref_logps fp32 [2 P] the frozen model's log-probabilities.
         logps[s] = sum over scored tokens of log softmax(logits)[target]
         m_i = beta * ((logps - ref_logps)[2i] - (logps - ref_logps)[2i + 1])
         loss = mean_i (1 - label_smoothing) softplus(-m_i) + label_smoothing softplus(m_i)
