@@ -447,24 +447,29 @@ struct OwnRow {
 //   * puts dS into its products in two bf16 parts.
 // dq of 2, 4 and 16 keys (among 130 tokens) is off by 4.0e-3, 3.0e-3, 2.2e-3 of its norm without the first; of 64 keys by 2.4e-3
 // without the second; with both by 1.7e-3, which is the rounding of dq alone.  Backward pass of 500 sequences of 64 tokens, 18
-// heads: 215 and 226 us.  For sequences of up to 512 keys the second part would make 64 x 512 tokens 354 -> 486 us.
-// The rule looks at the sequence's own keys alone: a padded row's gradients are as exact as the packed sequence's, whatever else
-// is in the call.
-constexpr int AG_FEW_KEYS = 64;
+// heads: 215 and 226 us.  The rule looks at the sequence's own keys alone: a padded row's gradients are as exact as the packed
+// sequence's, whatever else is in the call.
+// Of 65 to 512 keys dq and dk are off by 2.5e-3 and 2.4e-3, and with dS in two parts by 1.8e-3.  That would cost calls of many blocks
+// 14 to 18 % (backward pass, 18 heads: 160 x 200 tokens 278 and 318 us, 64 x 512 354 and 420), and costs those of few blocks 3 %
+// ("few rows" below; 8 x 512, 2 heads: 31.3 and 32.3), which have it.
+constexpr int AG_FEW_KEYS = 64, AG_SOME_KEYS = 512;
 
-// Masked sequences count 512 keys at a time and stop behind the 64th, so that all but very sparse masks cost one read (64 x 512
-// tokens with a mask, backward pass: 359 and 365 us).
-__device__ __forceinline__ bool few_keys(const unsigned char* mask, const Span& sp, int lane) {
-    if (!mask || sp.len <= AG_FEW_KEYS) return sp.len <= AG_FEW_KEYS;
+// The keys of a sequence that take part, or any number above `most` if there are more.  Masked sequences count 512 at a time, so that
+// all but very sparse masks cost one read (64 x 512 tokens with a mask, backward pass: 359 and 365 us).
+__device__ __forceinline__ int live_keys(const unsigned char* mask, const Span& sp, int lane, int most) {
+    if (!mask || sp.len <= AG_FEW_KEYS) return sp.len;  // of 64 tokens no more than that
     int n = 0;
-    for (int r0 = 0; r0 < sp.len && n <= AG_FEW_KEYS; r0 += 512) {
+    for (int r0 = 0; r0 < sp.len && n <= most; r0 += 512) {
         unsigned char m[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) m[i] = mask_byte(mask, sp.s0, r0 + 64 * i + lane, sp.len);
 #pragma unroll
         for (int i = 0; i < 8; ++i) n += __popcll(__ballot(m[i] != 0));
     }
-    return n <= AG_FEW_KEYS;
+    return n;
+}
+__device__ __forceinline__ bool few_keys(const unsigned char* mask, const Span& sp, int lane) {
+    return live_keys(mask, sp, lane, AG_FEW_KEYS) <= AG_FEW_KEYS;
 }
 
 // What the rounding of f to `a` leaves, rounded again: f is off by 2^-17 relative at most in the two parts together.
@@ -1105,8 +1110,8 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dq_fe
 #pragma unroll
         for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, nl)) * dp[r];
     };
-    const bool few = few_keys(mask, sp, lane);
-    if (few) {  // delta without the rounding of out, as in the large kernel
+    const int keys = live_keys(mask, sp, lane, AG_SOME_KEYS);
+    if (keys <= AG_FEW_KEYS) {  // delta without the rounding of out, as in the large kernel
         float more = 0.f;
         for_own_tiles<D>(k, v, mask, sp, head / group, ring, bias[wave], wave, lane, [&](int cur, const float* st) {
             products(cur, st);
@@ -1126,7 +1131,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dq_fe
         products(cur, st);
         const bf16x8 ds[2] = {pack8(e), pack8(e + 8)};  // 2^-8 relative at most, for the product with K
         mfma_tr<D, 0>(acc, ta, lds0 + cur, ds);
-        if (few) mfma_tr<D, 0>(acc, ta, lds0 + cur, rest_of(e, ds).b);
+        if (keys <= AG_SOME_KEYS) mfma_tr<D, 0>(acc, ta, lds0 + cur, rest_of(e, ds).b);
     });
     __syncthreads();
     join_rows<D>((float*)smem, acc, scale, wave, lane, dq.p + (sp.s0 + sp.first) * dq.tok + head * dq.head, dq.tok, sp.len - sp.first);
@@ -1203,7 +1208,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dkdv_
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(ring);
     const float c = scale * AG_LOG2E;
     if (wave < total) stage(0);
-    const bool few = few_keys(mask, sp, lane);
+    const bool some = live_keys(mask, sp, lane, AG_SOME_KEYS) <= AG_SOME_KEYS;
     for (int i = wave, j = 0; i < total; i += AG_WAVES, j ^= 1) {
         const int cur = j * SLOT;
         stat[wave][j][hi][l31] = next;
@@ -1222,7 +1227,7 @@ __global__ __launch_bounds__(AG_WAVES * 64, D == 64 ? 2 : 1) void attn_bwd_dkdv_
         mfma_tr<D, 0>(av, ta, lds0 + cur + TILE, p);
         const bf16x8 ds[2] = {pack8(f), pack8(f + 8)};  // the same, for the product with Q
         mfma_tr<D, 0>(ak, ta, lds0 + cur, ds);
-        if (few) mfma_tr<D, 0>(ak, ta, lds0 + cur, rest_of(f, ds).b);
+        if (some) mfma_tr<D, 0>(ak, ta, lds0 + cur, rest_of(f, ds).b);
     }
     if (!live) {
 #pragma unroll

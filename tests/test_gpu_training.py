@@ -576,6 +576,30 @@ def test_attention_gradients_of_few_keys_do_not_depend_on_the_rest_of_the_call(D
             within(a, b.expand_as(a), t, f"{name}, {len(args[0])} tokens, {args[0].shape[1]} heads")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_small_calls_keep_two_parts_up_to_512_keys(D, masked):
+    """dq and dk of 65 to 512 keys in few blocks, against 64 bits with the delta that the forward pass's rounded out gives.  What is
+    left is the rounding of the result and, were dS rounded once, one as large and independent of it: 1.41 times the former.
+    1.2 is asked of each sequence."""
+    live = [65, 130, 300, 512]
+    lens = [n + n // 3 if masked else n for n in live]  # with every fourth key masked as many take part
+    q, k, v, cu, cut, dout, g = attention_inputs(90 + D, lens, 2, 2, D)
+    mask = torch.arange(len(q), device="cuda") % 4 != 3 if masked else None
+    got = attention_all(q, k, v, cut, dout, mask=mask)
+    scale = D ** -0.5
+    for a, b in zip(cu, cu[1:]):
+        keep = torch.ones(b - a, dtype=torch.bool, device="cuda") if mask is None else mask[a:b]
+        assert 64 < keep.sum() <= 512
+        for h in range(2):
+            Q, K, V, dO, O = (t[a:b, h].double() for t in (q, k, v, dout, got[0]))
+            P = (Q @ K.t() * scale).masked_fill(~keep, -math.inf).softmax(-1)
+            dS = scale * P * (dO @ V.t() - (dO * O).sum(-1, keepdim=True))
+            for x, exact, name in ((got[2], dS @ K, "dq"), (got[3], dS.t() @ Q, "dk")):
+                rounding = (exact.bfloat16().double() - exact).norm()
+                assert (x[a:b, h].double() - exact).norm() <= 1.2 * rounding, f"{name} of {b - a} tokens"
+
+
 def test_attention_rising_and_falling_scores():
     """Keys whose scores rise from tile to tile by far more than the reference point may lag, and fall again; large values."""
     N = 64 * 9
